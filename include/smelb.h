@@ -417,6 +417,34 @@ int smelb_lm_logits(const void* h, int64_t N, int64_t H, const void* w, const vo
                     int64_t vocab_chunk, float softcap, float* out, void* workspace, int64_t workspace_bytes,
                     void* stream);
 
+/* ---------------------------------------------------------------------------------------------------- routing losses
+ * No counterpart in the reference (its stats callback, smel/moe.py:258-259, hands out the same tables).
+ * Balance loss of the routing tables probs (fp32 [T, E], row pitch ld elements) and topi (int64 [T, K]): sequence s
+ * holds the rows cu_seqlens[s] .. cu_seqlens[s + 1] - 1 (device int32 [S + 1], not decreasing; NULL: one sequence of all
+ * T rows, S = 1), mask (device uint8 [T], may be NULL) keeps the rows that are not 0. With n_s kept rows, c[s][e] their
+ * choices of e and P[s][e] the sum of their probs[.][e]:
+ *   loss (fp32 [1]) = 1/S' sum_s E / (K n_s^2) sum_e c[s][e] P[s][e] over the S' sequences with n_s > 0 (0 without any)
+ *   counts (int64 [S][E]) = c;  coef (fp32 [S * E + 1]): the gradient's rows, for smelb_balance_loss_bwd.
+ * Rows outside every sequence and rows the mask drops are not read and have a zero gradient. Indices outside [0, E)
+ * are not counted and recorded in the status word. E <= 512, K <= 32. workspace: 256-byte aligned,
+ * smelb_balance_workspace_bytes(T, E, S, 0) bytes. Equal inputs give equal bits. */
+int64_t smelb_balance_workspace_bytes(int64_t T, int64_t E, int64_t S, int usage);
+int smelb_balance_loss_fwd(const float* probs, int64_t ld, const int64_t* topi, const uint8_t* mask,
+                           const int32_t* cu_seqlens, int64_t S, int64_t T, int64_t E, int64_t K, float* loss,
+                           int64_t* counts, float* coef, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* dprobs (fp32 [T, E], contiguous) = go[0] * d loss / d probs; go: device fp32 [1]; coef, mask and cu_seqlens as in the
+ * forward. Every row is written. */
+int smelb_balance_loss_bwd(const float* coef, const float* go, const uint8_t* mask, const int32_t* cu_seqlens,
+                           int64_t S, int64_t T, int64_t E, float* dprobs, void* stream);
+
+/* Per-expert usage of T routed tokens over the rows that mask keeps: counts (int64 [E]) choices, prob_mass (fp32 [E])
+ * sum of probs, weight_mass (fp32 [E]) sum of the routing weights topv (bf16, or fp32 if topv_fp32, [T, K]) of the
+ * expert's choices. workspace: 256-byte aligned, smelb_balance_workspace_bytes(T, E, 1, 1) bytes. */
+int smelb_expert_usage(const float* probs, int64_t ld, const void* topv, int topv_fp32, const int64_t* topi,
+                       const uint8_t* mask, int64_t T, int64_t E, int64_t K, int64_t* counts, float* prob_mass,
+                       float* weight_mass, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Instrumentation. smelb_launch_count: kernels launched by this library so far (all entry points).
  * smelb_gemm_timing(1) records a CUDA event pair on the launching stream around every expert-GEMM launch;
  * smelb_gemm_timing_read synchronizes on them and returns the summed duration (ms) and the number of launches

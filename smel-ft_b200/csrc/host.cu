@@ -39,6 +39,17 @@ int* device_status(int dev) {
   return g_status[dev];
 }
 
+int* device_status_on(int dev, cudaStream_t st) {
+  if (dev < 0 || dev >= 64) return nullptr;
+  {
+    std::lock_guard<std::mutex> lk(g_mu);
+    if (g_status[dev]) return g_status[dev];
+  }
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(st, &cap) != cudaSuccess || cap != cudaStreamCaptureStatusNone) return nullptr;
+  return device_status(dev);
+}
+
 int num_sms(int dev) {
   if (dev < 0 || dev >= 64) return 148;
   if (!g_sms[dev]) {

@@ -11,6 +11,9 @@ namespace smelb {
 
 // 4-byte device word the kernels record wait timeouts in (allocated once per device)
 int* device_status(int dev);
+// The same for a launch on `st`: null (nothing is recorded) when the word does not exist yet and the stream is being
+// captured, where it cannot be allocated.
+int* device_status_on(int dev, cudaStream_t st);
 
 // Instrumentation: number of kernels launched by the library, and optional CUDA-event timing of the GEMM launches.
 void count_launch();

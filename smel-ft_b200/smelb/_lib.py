@@ -131,6 +131,12 @@ SIGNATURES = {
                                  c_vp, c_vp, c_vp, c_i64, c_vp]),
     "smelb_lm_logits_workspace_bytes": (c_i64, [c_i64, c_i64, c_i64, c_i32]),
     "smelb_lm_logits": (c_i32, [c_vp, c_i64, c_i64, c_vp, c_vp, c_vp, c_i64, c_i64, c_f32, c_vp, c_vp, c_i64, c_vp]),
+    "smelb_balance_workspace_bytes": (c_i64, [c_i64, c_i64, c_i64, c_i32]),
+    "smelb_balance_loss_fwd": (c_i32, [c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp,
+                                       c_i64, c_vp]),
+    "smelb_balance_loss_bwd": (c_i32, [c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp]),
+    "smelb_expert_usage": (c_i32, [c_vp, c_i64, c_vp, c_i32, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp,
+                                   c_i64, c_vp]),
     "smelb_moe_layer_size": (ctypes.c_size_t, []),
     "smelb_launch_count": (ctypes.c_longlong, []),
     "smelb_gemm_timing": (c_i32, [c_i32]),
@@ -169,6 +175,16 @@ def call(name, *args):
     if torch.cuda.is_available():
         lib.smelb_set_device(torch.cuda.current_device())
     rc = getattr(lib, name)(*args)
+    if rc != 0:
+        raise SmelbError(f"{name}: {ERRORS.get(rc, rc)}: {last_error()}")
+
+
+def call_on(device, name, *args):
+    """Call an entry point with `device`, the device of its tensors, current for the call."""
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return call_on(device, name, *args)
+    rc = getattr(load(), name)(*args)
     if rc != 0:
         raise SmelbError(f"{name}: {ERRORS.get(rc, rc)}: {last_error()}")
 
