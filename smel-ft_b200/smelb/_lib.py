@@ -65,6 +65,11 @@ class MoELayerStruct(ctypes.Structure):
     _fields_ = _LAYER_FIELDS
 
 
+class MuonTensor(ctypes.Structure):
+    """struct smelb_muon_tensor."""
+    _fields_ = [("p", c_vp), ("g", c_vp), ("m", c_vp), ("batch", c_i64), ("rows", c_i64), ("cols", c_i64)]
+
+
 # exported symbol -> (restype, argtypes)
 SIGNATURES = {
     "smelb_version": (c_i32, []),
@@ -137,6 +142,9 @@ SIGNATURES = {
     "smelb_balance_loss_bwd": (c_i32, [c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp]),
     "smelb_expert_usage": (c_i32, [c_vp, c_i64, c_vp, c_i32, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp,
                                    c_i64, c_vp]),
+    "smelb_orthogonalize": (c_i32, [c_vp, c_i32, c_i64, c_i64, c_i64, c_i32, c_vp, ctypes.c_double, c_vp, c_vp]),
+    "smelb_muon_step": (c_i32, [ctypes.POINTER(MuonTensor), c_i64, c_i32, ctypes.c_double, ctypes.c_double, c_i32,
+                                ctypes.c_double, c_i32, c_i32, c_vp, ctypes.c_double, c_vp]),
     "smelb_moe_layer_size": (ctypes.c_size_t, []),
     "smelb_launch_count": (ctypes.c_longlong, []),
     "smelb_gemm_timing": (c_i32, [c_i32]),
