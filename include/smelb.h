@@ -450,23 +450,29 @@ int smelb_expert_usage(const float* probs, int64_t ld, const void* topv, int top
  * min(rows, cols) <= 64 (the width of a LoRA block): X = x / (|x|_F + eps), then `steps` (1..16) times
  * X <- a X + b (X X^T) X + c (X X^T)^2 X on the short side, with (a, b, c) = coefficients[3 s .. 3 s + 2] (host array) of
  * step s. out may alias x. dtype 0: fp32, 1: bf16 (x and out alike). Sums and the products of the short side are fp64.
- * A matrix of zeros gives zeros; one that holds an infinity or NaN gives NaN and leaves the others alone. */
+ * A matrix of zeros gives zeros; one that holds an infinity or NaN gives NaN and leaves the others alone. workspace:
+ * 256-byte aligned, smelb_orthogonalize_workspace_bytes bytes (0 for short sides up to 32 unless they are very long). */
+int64_t smelb_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols);
 int smelb_orthogonalize(const void* x, int dtype, int64_t batch, int64_t rows, int64_t cols, int steps,
-                        const double* coefficients, double eps, void* out, void* stream);
+                        const double* coefficients, double eps, void* out, void* workspace, int64_t workspace_bytes,
+                        void* stream);
 
 /* A Muon step of n tensors (host array), each a batch of [rows, cols] matrices as for smelb_orthogonalize, in place:
  *   m <- momentum m + (1 - momentum) g;  u = nesterov ? momentum m + (1 - momentum) g : m
  *   p <- p (1 - lr weight_decay) - lr f orthogonalize(u),  f = sqrt(max(1, rows / cols)) (adjust 0) or
  *   0.2 sqrt(max(rows, cols)) (adjust 1).
- * p and g of the dtype (0: fp32, 1: bf16), m fp32. No tensor may overlap another. */
+ * p and g of the dtype (0: fp32, 1: bf16), m fp32. No tensor may overlap another. workspace: 256-byte aligned,
+ * smelb_muon_workspace_bytes bytes (it reads the tensors' sizes alone; -1 for sizes that are refused). */
 typedef struct smelb_muon_tensor {
   void* p;
   const void* g;
   float* m;
   int64_t batch, rows, cols;
 } smelb_muon_tensor;
+int64_t smelb_muon_workspace_bytes(const smelb_muon_tensor* tensors, int64_t n);
 int smelb_muon_step(const smelb_muon_tensor* tensors, int64_t n, int dtype, double lr, double momentum, int nesterov,
-                    double weight_decay, int adjust, int steps, const double* coefficients, double eps, void* stream);
+                    double weight_decay, int adjust, int steps, const double* coefficients, double eps, void* workspace,
+                    int64_t workspace_bytes, void* stream);
 
 /* Instrumentation. smelb_launch_count: kernels launched by this library so far (all entry points).
  * smelb_gemm_timing(1) records a CUDA event pair on the launching stream around every expert-GEMM launch;

@@ -7,13 +7,13 @@
 //   S = a I + b G + c G^2;   P <- S P;   G <- S G S.
 // Precision. The steps grow a singular value near zero by a^steps (485 for the usual polynomial), and an error delta in
 // G moves the result by delta / sigma^2, so gradients of low rank (few tokens reached the expert) come out up to 3e-4
-// off when G is held in fp32. G and the d x d matrices are fp64, on the fp64 matrix instruction (m8n8k4): at d = 16
-// that is 4 operations per byte of x, below the card's 5.7 (37 TFLOP/s over 6.4 TB/s), so it costs no time on long
-// factors.
+// off when G is held in fp32. G and the d x d matrices are fp64, on the fp64 matrix instruction (m8n8k4); the product
+// with x is fp32 where P is small and fp64 elsewhere.
 //
-// One cluster of 1, 2, 4 or 8 blocks per matrix. A block keeps its slice of the long side in shared memory as fp32
-// [d][columns] whatever the layout in memory (a slice that does not fit is read a second time); partial Gram matrices
-// are added over the cluster in rank order through distributed shared memory, and each block forms P for itself.
+// Two ways, by the size of a matrix:
+//   resident  a cluster of 1 to 8 blocks holds one matrix in shared memory and reads it once (ortho_kernel)
+//   split     many blocks add partial Gram matrices of one matrix, one block forms P, many blocks apply it
+//             (gram_kernel, form_kernel, product_kernel); x is read twice
 #include <algorithm>
 
 #include "common.cuh"
@@ -24,49 +24,59 @@ namespace smelb {
 namespace {
 
 constexpr int kThreads = 256, kWarps = 8;
-constexpr int kMaxSteps = 16, kMaxTensors = 64, kMaxD = 64;
+constexpr int kMaxSteps = 16, kMaxTensors = 48, kMaxD = 64;
 
 struct Tensor {
-  void* p;        // parameter (momentum step) or output
-  const void* g;  // gradient or input
-  float* m;       // momentum buffer
+  void* p;          // parameter (momentum step) or output
+  const void* g;    // gradient or input
+  float* m;         // momentum buffer
   long long start;  // matrices before this tensor's
-  int d, L;       // short and long side
-  int tall;       // memory is [L][d] (else [d][L])
-  float step;     // lr * shape factor
+  int d, L;         // short and long side
+  int tall;         // memory is [L][d] (else [d][L])
+  uint32_t by_d;    // 2^32 / d + 1: division by d
+  float step;       // lr * shape factor
 };
 
 struct Args {
   Tensor t[kMaxTensors];
-  int n, steps, cluster, cap;  // cap: columns that a block holds at once
+  int n, steps;
+  int blocks;        // blocks of one matrix
+  int cap;           // columns that a block holds at once (a multiple of 32)
+  uint32_t by_v[2];  // 2^32 / (cap / 4) + 1 and 2^32 / (cap / 8) + 1
   float mu, omu, decay;  // omu: 1 - momentum, from 64 bits
   int nesterov;
   double eps;
+  double* gram;  // split: [matrix][block][PART] partial Gram matrices
+  double* form;  // split: [matrix][NT * NT * 64 + 1] P and whether it is plain
   double coef[kMaxSteps][3];
 };
 
+// d x d matrices are NT x NT tiles of 8 x 8 doubles, row-major in the tile, so a lane's two accumulators of the matrix
+// instruction (row lane / 4, columns 2 (lane % 4) + e) are 16 bytes at 2 lane. Read with those indices they are also the
+// instruction's operands when the sum over k takes the columns in the order 2 c + e (c the lane's place, e the step):
+// as the left one directly, as the right one because the matrices are symmetric. A product of tiles is two 16-byte
+// loads for two instructions, without a shuffle.
 template <int NT>
 struct Dims {
-  static constexpr int D = NT * 8, LDM = D + 4;            // row pitch of the fp64 matrices: conflict-free fragments
-  static constexpr int TILES = NT * (NT + 1) / 2;          // tiles of the upper triangle
-  static constexpr int GROUPS = NT == 8 ? 4 : 1;           // tile groups among the warps (accumulators in registers)
-  static constexpr int KG = kWarps / GROUPS;               // warps that split the columns
-  static constexpr int BUFS = KG < 4 ? KG : 4;             // partial Gram matrices in shared memory at once
-  static constexpr int MAT = D * LDM;                      // doubles of one matrix
-  static constexpr int PART = TILES * 64;                  // doubles of one packed upper triangle
-  // G, S, P, V, then this block's part of the Gram matrix; the warps' partial sums alias S, P and V
-  static constexpr int WORK = (3 * MAT > BUFS * PART ? 3 * MAT : BUFS * PART);
-  static constexpr long long kFixed = (long long)(MAT + WORK + PART) * 8;
+  static constexpr int D = NT * 8;
+  static constexpr int TILES = NT * (NT + 1) / 2;       // tiles of the upper triangle
+  static constexpr int GROUPS = NT == 8 ? 4 : 1;        // tile groups among the warps (accumulators in registers)
+  static constexpr int ACC = GROUPS == 1 ? TILES : NT + 1;  // tiles of a group
+  static constexpr int KG = kWarps / GROUPS;            // warps that split the columns
+  static constexpr int BUFS = KG < 4 ? KG : 4;          // partial Gram matrices in shared memory at once
+  static constexpr int MAT = NT * NT * 64;              // doubles of one matrix
+  static constexpr int PART = TILES * 64;               // doubles of one packed upper triangle
+  static constexpr int WORK = 4 * MAT > BUFS * PART ? 4 * MAT : BUFS * PART;  // S, V and two P; partial sums before
 };
 
-// Column pitch 8 mod 32 and columns of rows 4-7 (mod 8) shifted by four: the fragments of the Gram product (8 rows x 4
-// columns) and of the product with P (4 rows x 8 columns) then both touch 32 different banks.
-__device__ __forceinline__ int xat(int i, int j, int ld) { return i * ld + (j ^ (i & 4)); }
+// Pitch of the columns in shared memory: 4 mod 32, so the operands of the Gram product (8 rows x 4 columns) and of the
+// product with P (rows 2 c + e, 8 columns) both touch 32 different banks.
+__host__ __device__ constexpr int pitch(int cap) { return cap + 4; }
 
 __device__ __forceinline__ void dmma(double (&c)[2], double a, double b) {
-  asm volatile("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0, %1}, {%2}, {%3}, {%0, %1};"
-               : "+d"(c[0]), "+d"(c[1])
-               : "d"(a), "d"(b));
+  asm("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0, %1}, {%2}, {%3}, {%0, %1};"
+      : "+d"(c[0]), "+d"(c[1])
+      : "d"(a), "d"(b));
 }
 
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
@@ -84,59 +94,231 @@ __device__ __forceinline__ float to_f(bf16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(bf16* p, float v) { *p = __float2bfloat16_rn(v); }
 
-// One element of the input: the gradient, or the momentum update, whose new buffer is written when `first`.
-template <typename T, bool MUON>
-__device__ __forceinline__ float element(const Args& a, const Tensor& t, long long at, bool first) {
-  const float g = to_f(reinterpret_cast<const T*>(t.g)[at]);
-  if (!MUON) return g;
-  float m = t.m[at];
-  if (first) {
-    m = fmaf(a.mu, m, a.omu * g);
-    t.m[at] = m;
-  }
+// The momentum update u of one element from its gradient and buffer; `first` (the buffer is still the old one) renews it.
+__device__ __forceinline__ float update(const Args& a, float g, float& m, bool first) {
+  if (first) m = fmaf(a.mu, m, a.omu * g);
   return a.nesterov ? fmaf(a.mu, m, a.omu * g) : m;
 }
 
-// Columns [j0, j0 + w) into x, zeros up to the next multiple of 8.
-template <typename T, bool MUON>
-__device__ void load_slice(const Args& a, const Tensor& t, long long base, int j0, int w, float* x, int ld, int D,
-                           bool first) {
+// 16 bytes of T as floats and back.
+template <typename T>
+struct Vec {
+  static constexpr int N = 16 / sizeof(T);
+  float v[N];
+};
+__device__ __forceinline__ void unpack(const uint4& r, Vec<float>& o) {
+  o.v[0] = __uint_as_float(r.x);
+  o.v[1] = __uint_as_float(r.y);
+  o.v[2] = __uint_as_float(r.z);
+  o.v[3] = __uint_as_float(r.w);
+}
+__device__ __forceinline__ void unpack(const uint4& r, Vec<bf16>& o) {
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    o.v[2 * k] = __uint_as_float(w[k] << 16);
+    o.v[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ uint4 repack(const Vec<float>& o) {
+  return make_uint4(__float_as_uint(o.v[0]), __float_as_uint(o.v[1]), __float_as_uint(o.v[2]), __float_as_uint(o.v[3]));
+}
+__device__ __forceinline__ uint4 repack(const Vec<bf16>& o) {
+  uint32_t w[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(o.v[2 * k], o.v[2 * k + 1]);
+    w[k] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+
+// The vectors of N elements of a block's columns [j0, j0 + w): vector q of a wide matrix is row q / (cap / N), columns from
+// N (q % (cap / N)); a tall matrix is contiguous, element e of it is (i, j) = (e % d, e / d).
+template <int N>
+struct Place {
+  int i, j;
+  long long at;  // offset in memory from column j0
+  bool live;
+  __device__ __forceinline__ Place(const Args& a, const Tensor& t, int w, int q) {
+    if (t.tall) {
+      const int e = q * N;
+      j = (int)__umulhi((uint32_t)e, t.by_d);
+      i = e - j * t.d;
+      at = e;
+      live = j < w;
+    } else {
+      i = (int)__umulhi((uint32_t)q, a.by_v[N == 8]);
+      j = (q - i * (a.cap / N)) * N;
+      at = (long long)i * t.L + j;
+      live = i < t.d && j < w;
+    }
+  }
+};
+template <int N>
+__device__ __forceinline__ int places(const Args& a, const Tensor& t, int w) {
+  return t.tall ? w * t.d / N : t.d * (a.cap / N);
+}
+
+// The N elements of a vector: v -> x (PUT) or x -> v.
+template <bool PUT, int N>
+__device__ __forceinline__ void move(const Tensor& t, const Place<N>& at, float* x, int ld, float (&v)[N]) {
   if (t.tall) {
-    for (int q = threadIdx.x; q < w * t.d; q += kThreads) {
-      const int j = q / t.d, i = q - j * t.d;
-      x[xat(i, j, ld)] = element<T, MUON>(a, t, base + (long long)j0 * t.d + q, first);
+    int i = at.i;
+    float* c = x + at.j;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      if (PUT) c[i * ld] = v[k];
+      else v[k] = c[i * ld];
+      if (++i == t.d) {
+        i = 0;
+        ++c;
+      }
     }
   } else {
-    for (int i = 0; i < t.d; ++i)
-      for (int j = threadIdx.x; j < w; j += kThreads)
-        x[xat(i, j, ld)] = element<T, MUON>(a, t, base + (long long)i * t.L + j0 + j, first);
+#pragma unroll
+    for (int k = 0; k < N; k += 4) {
+      float4* c = reinterpret_cast<float4*>(x + at.i * ld + at.j + k);
+      if (PUT) {
+        *c = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+      } else {
+        const float4 o = *c;
+        v[k] = o.x;
+        v[k + 1] = o.y;
+        v[k + 2] = o.z;
+        v[k + 3] = o.w;
+      }
+    }
+  }
+}
+
+// Whether the vectors of a slice start on 16 bytes and end with it.
+template <typename T, bool MUON>
+__device__ __forceinline__ bool vectors(const Tensor& t, long long base, int w) {
+  constexpr int N = 16 / sizeof(T);
+  const uintptr_t at = (uintptr_t)(reinterpret_cast<const T*>(t.g) + base) |
+                       (uintptr_t)(reinterpret_cast<T*>(t.p) + base) | (MUON ? (uintptr_t)(t.m + base) : 0);
+  return (at & 15) == 0 && (t.tall ? (w * t.d) % N == 0 : t.L % N == 0 && w % N == 0);
+}
+
+// Columns [j0, j0 + w) (j0 a multiple of 8) into x, zeros up to the next multiple of 8 and in the rows that fill the
+// tiles. `first`: the momentum buffer is still the old one.
+template <int NT, typename T, bool MUON>
+__device__ __forceinline__ void load_slice(const Args& a, const Tensor& t, long long base, int j0, int w, float* x,
+                                           int ld, bool first) {
+  constexpr int N = Vec<T>::N, U = MUON && N == 8 ? 2 : 4;  // vectors in flight per thread
+  base += t.tall ? (long long)j0 * t.d : j0;
+  const T* g = reinterpret_cast<const T*>(t.g) + base;
+  float* m = MUON ? t.m + base : nullptr;
+  if (vectors<T, MUON>(t, base, w)) {
+    const int end = places<N>(a, t, w);
+    for (int q0 = threadIdx.x; q0 < end; q0 += kThreads * U) {
+      uint4 rg[U], rm[U][N / 4];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const Place<N> at(a, t, w, q0 + u * kThreads);
+        if (at.live) {
+          rg[u] = __ldg(reinterpret_cast<const uint4*>(g + at.at));
+          if (MUON) {
+#pragma unroll
+            for (int k = 0; k < N / 4; ++k) rm[u][k] = *reinterpret_cast<const uint4*>(m + at.at + 4 * k);
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const Place<N> at(a, t, w, q0 + u * kThreads);
+        if (at.live) {
+          Vec<T> v;
+          unpack(rg[u], v);
+          if (MUON) {
+#pragma unroll
+            for (int k = 0; k < N / 4; ++k) {
+              Vec<float> b;
+              unpack(rm[u][k], b);
+#pragma unroll
+              for (int l = 0; l < 4; ++l) v.v[4 * k + l] = update(a, v.v[4 * k + l], b.v[l], first);
+              if (first) *reinterpret_cast<uint4*>(m + at.at + 4 * k) = repack(b);
+            }
+          }
+          move<true>(t, at, x, ld, v.v);
+        }
+      }
+    }
+  } else {
+    for (int q = threadIdx.x; q < w * t.d; q += kThreads) {
+      const int i = t.tall ? q % t.d : q / w, j = t.tall ? q / t.d : q % w;
+      const long long at = t.tall ? (long long)q : (long long)i * t.L + j;
+      float v = to_f(g[at]);
+      if (MUON) {
+        float b = m[at];
+        v = update(a, v, b, first);
+        if (first) m[at] = b;
+      }
+      x[i * ld + j] = v;
+    }
   }
   const int w8 = (w + 7) & ~7;
-  for (int i = threadIdx.x >> 3; i < t.d; i += kThreads / 8) {
-    const int j = (w8 - 8) + (threadIdx.x & 7);
-    if (j >= w) x[xat(i, j, ld)] = 0.f;
-  }
-  for (int q = threadIdx.x; q < (D - t.d) * w8; q += kThreads) x[xat(t.d + q / w8, q % w8, ld)] = 0.f;
+  if (w < w8)
+    for (int i = threadIdx.x >> 3; i < t.d; i += kThreads / 8) {
+      const int j = (w8 - 8) + (threadIdx.x & 7);
+      if (j >= w) x[i * ld + j] = 0.f;
+    }
+  if (t.d < NT * 8)
+    for (int i = t.d; i < NT * 8; ++i)
+      for (int j = threadIdx.x; j < w8; j += kThreads) x[i * ld + j] = 0.f;
+}
+
+// The result o at a place whose present value is p.
+template <bool MUON>
+__device__ __forceinline__ float result(const Args& a, const Tensor& t, float o, float p) {
+  return MUON ? fmaf(-t.step, o, p * a.decay) : o;
 }
 
 template <typename T, bool MUON>
-__device__ __forceinline__ void emit(const Args& a, const Tensor& t, long long at, float o) {
-  T* p = reinterpret_cast<T*>(t.p) + at;
-  put(p, MUON ? fmaf(-t.step, o, to_f(*p) * a.decay) : o);
-}
-
-template <typename T, bool MUON>
-__device__ void store_slice(const Args& a, const Tensor& t, long long base, int j0, int w, const float* x, int ld) {
-  if (t.tall) {
-    for (int q = threadIdx.x; q < w * t.d; q += kThreads) {
-      const int j = q / t.d, i = q - j * t.d;
-      emit<T, MUON>(a, t, base + (long long)j0 * t.d + q, x[xat(i, j, ld)]);
+__device__ __forceinline__ void store_slice(const Args& a, const Tensor& t, long long base, int j0, int w, float* x,
+                                            int ld) {
+  constexpr int N = Vec<T>::N, U = 4;
+  base += t.tall ? (long long)j0 * t.d : j0;
+  T* p = reinterpret_cast<T*>(t.p) + base;
+  if (vectors<T, MUON>(t, base, w)) {
+    const int end = places<N>(a, t, w);
+    for (int q0 = threadIdx.x; q0 < end; q0 += kThreads * U) {
+      uint4 rp[U];
+      if (MUON) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const Place<N> at(a, t, w, q0 + u * kThreads);
+          if (at.live) rp[u] = *reinterpret_cast<const uint4*>(p + at.at);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const Place<N> at(a, t, w, q0 + u * kThreads);
+        if (at.live) {
+          Vec<T> v, was{};
+          if (MUON) unpack(rp[u], was);
+          move<false>(t, at, x, ld, v.v);
+#pragma unroll
+          for (int k = 0; k < N; ++k) v.v[k] = result<MUON>(a, t, v.v[k], was.v[k]);
+          *reinterpret_cast<uint4*>(p + at.at) = repack(v);
+        }
+      }
     }
   } else {
-    for (int i = 0; i < t.d; ++i)
-      for (int j = threadIdx.x; j < w; j += kThreads)
-        emit<T, MUON>(a, t, base + (long long)i * t.L + j0 + j, x[xat(i, j, ld)]);
+    for (int q = threadIdx.x; q < w * t.d; q += kThreads) {
+      const int i = t.tall ? q % t.d : q / w, j = t.tall ? q / t.d : q % w;
+      T* at = p + (t.tall ? (long long)q : (long long)i * t.L + j);
+      put(at, result<MUON>(a, t, x[i * ld + j], MUON ? to_f(*at) : 0.f));
+    }
   }
+}
+
+// Tile (i, j), i <= j, of the packed upper triangle.
+template <int NT>
+__host__ __device__ constexpr int tri(int i, int j) {
+  return i * NT - i * (i - 1) / 2 + j - i;
 }
 
 // Tile rows of a warp's tile group: all of them, or rows Q and 7 - Q of eight (nine tiles in every group).
@@ -148,188 +330,51 @@ __host__ __device__ constexpr bool in_group(int i) {
 // acc += the group's tiles of X X^T over columns 4 k .. 4 k + 3 for k = kg, kg + KG, ... The fragment of rows 8 i ..
 // 8 i + 7 is the same as left and as right operand.
 template <int NT, int Q>
-__device__ __forceinline__ void gram(const float* x, int ld, int w, int kg, double (&acc)[Dims<NT>::TILES][2]) {
-  const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+__device__ __forceinline__ void gram(const float* x, int ld, int w, int kg, double (&acc)[Dims<NT>::ACC][2]) {
+  const int lane = threadIdx.x & 31;
+  const float* p = x + (lane >> 2) * ld + (lane & 3);
+#pragma unroll 2
   for (int k = kg * 4; k < w; k += Dims<NT>::KG * 4) {
     double f[NT];
 #pragma unroll
-    for (int i = 0; i < NT; ++i) f[i] = x[xat(8 * i + r, k + c, ld)];
+    for (int i = 0; i < NT; ++i) f[i] = p[8 * i * ld + k];
     int n = 0;
 #pragma unroll
     for (int i = 0; i < NT; ++i)
+      if (in_group<NT, Q>(i)) {
 #pragma unroll
-      for (int j = i; j < NT; ++j, ++n)
-        if (in_group<NT, Q>(i)) dmma(acc[n], f[i], f[j]);
+        for (int j = i; j < NT; ++j) dmma(acc[n++], f[i], f[j]);
+      }
   }
 }
 
-// Adds or writes the group's tiles into a packed upper triangle.
+// The group's tiles to or from (added) a packed upper triangle.
 template <int NT, int Q, bool ADD>
-__device__ __forceinline__ void pack(double* part, double (&acc)[Dims<NT>::TILES][2]) {
+__device__ __forceinline__ void pack(double* part, double (&acc)[Dims<NT>::ACC][2]) {
   const int lane = threadIdx.x & 31;
   int n = 0;
 #pragma unroll
   for (int i = 0; i < NT; ++i)
+    if (in_group<NT, Q>(i)) {
 #pragma unroll
-    for (int j = i; j < NT; ++j, ++n)
-      if (in_group<NT, Q>(i)) {
-        double* d = part + n * 64 + lane * 2;
+      for (int j = i; j < NT; ++j, ++n) {
+        double2* d = reinterpret_cast<double2*>(part + tri<NT>(i, j) * 64 + lane * 2);
         if (ADD) {
-          acc[n][0] += d[0];
-          acc[n][1] += d[1];
+          acc[n][0] += d->x;
+          acc[n][1] += d->y;
         } else {
-          d[0] = acc[n][0];
-          d[1] = acc[n][1];
+          *d = make_double2(acc[n][0], acc[n][1]);
         }
       }
-}
-
-// c = rows 8 i .. of A times columns 8 j .. of B, both symmetric.
-template <int NT>
-__device__ __forceinline__ void product(const double* A, const double* B, int i, int j, double (&c)[2]) {
-  constexpr int LDM = Dims<NT>::LDM;
-  const int lane = threadIdx.x & 31;
-  const double* pa = A + (8 * i + (lane >> 2)) * LDM + (lane & 3);
-  const double* pb = B + (8 * j + (lane >> 2)) * LDM + (lane & 3);
-  c[0] = c[1] = 0.0;
-#pragma unroll
-  for (int k = 0; k < NT * 2; ++k) dmma(c, pa[4 * k], pb[4 * k]);
-}
-
-// Writes a tile and its mirror image.
-template <int NT>
-__device__ __forceinline__ void put_tile(double* M, int i, int j, const double (&c)[2]) {
-  constexpr int LDM = Dims<NT>::LDM;
-  const int lane = threadIdx.x & 31, r = 8 * i + (lane >> 2), k = 8 * j + 2 * (lane & 3);
-  M[r * LDM + k] = c[0];
-  M[r * LDM + k + 1] = c[1];
-  if (i != j) {
-    M[k * LDM + r] = c[0];
-    M[(k + 1) * LDM + r] = c[1];
-  }
-}
-
-// Tile n of the upper triangle.
-template <int NT>
-__device__ __forceinline__ void tile_of(int n, int& i, int& j) {
-  i = 0;
-  while (n >= NT - i) n -= NT - i++;
-  j = i + n;
-}
-
-// From the Gram matrix G (unscaled) to P with P x = the polynomial of x; leaves P in M[2].
-template <int NT>
-__device__ void iterate(const Args& a, double* G, double* S, double* P, double* V) {
-  using D_ = Dims<NT>;
-  constexpr int LDM = D_::LDM, PER = (D_::TILES + kWarps - 1) / kWarps;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  double tr = 0.0;
-  for (int i = 0; i < D_::D; ++i) tr += G[i * LDM + i];
-  const double inv = 1.0 / (sqrt(tr) + a.eps);
-  double sc = inv * inv;  // the first step's G still has to be scaled by it
-  for (int step = 0; step < a.steps; ++step) {
-    const double ca = a.coef[step][0], cb = a.coef[step][1] * sc, cc = a.coef[step][2] * sc * sc;
-    const bool last = step + 1 == a.steps;
-    for (int n = warp; n < D_::TILES; n += kWarps) {
-      int i, j;
-      tile_of<NT>(n, i, j);
-      double c[2];
-      product<NT>(G, G, i, j, c);
-      const int r = 8 * i + (lane >> 2), k = 8 * j + 2 * (lane & 3);
-      c[0] = cb * G[r * LDM + k] + cc * c[0] + (r == k ? ca : 0.0);
-      c[1] = cb * G[r * LDM + k + 1] + cc * c[1] + (r == k + 1 ? ca : 0.0);
-      put_tile<NT>(S, i, j, c);
-      if (step == 0) put_tile<NT>(P, i, j, c);
     }
-    __syncthreads();
-    double np[PER][2], nv[PER][2];
-#pragma unroll
-    for (int q = 0; q < PER; ++q) {
-      const int n = warp + q * kWarps;
-      if (n < D_::TILES) {
-        int i, j;
-        tile_of<NT>(n, i, j);
-        if (step) product<NT>(S, P, i, j, np[q]);
-        if (!last) product<NT>(S, G, i, j, nv[q]);
-      }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int q = 0; q < PER; ++q) {
-      const int n = warp + q * kWarps;
-      if (n < D_::TILES) {
-        int i, j;
-        tile_of<NT>(n, i, j);
-        if (step) put_tile<NT>(P, i, j, np[q]);
-        if (!last) put_tile<NT>(V, i, j, nv[q]);
-      }
-    }
-    __syncthreads();
-    if (!last) {
-      for (int n = warp; n < D_::TILES; n += kWarps) {
-        int i, j;
-        tile_of<NT>(n, i, j);
-        double c[2];
-        product<NT>(S, V, i, j, c);
-        c[0] *= sc;
-        c[1] *= sc;
-        put_tile<NT>(G, i, j, c);
-      }
-      __syncthreads();
-    }
-    sc = 1.0;
-  }
-  for (int i = threadIdx.x; i < D_::D * D_::D; i += kThreads) P[(i / D_::D) * LDM + i % D_::D] *= inv;
-  __syncthreads();
 }
 
-// x <- P x in place: a warp owns eight columns at a time.
 template <int NT>
-__device__ void apply(const double* P, float* x, int ld, int w) {
-  constexpr int LDM = Dims<NT>::LDM;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-  for (int j = warp * 8; j < w; j += kWarps * 8) {
-    double b[NT * 2];
-#pragma unroll
-    for (int k = 0; k < NT * 2; ++k) b[k] = x[xat(4 * k + c, j + r, ld)];
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      double o[2] = {0.0, 0.0};
-#pragma unroll
-      for (int k = 0; k < NT * 2; ++k) dmma(o, P[(8 * i + r) * LDM + 4 * k + c], b[k]);
-      *reinterpret_cast<float2*>(x + xat(8 * i + r, j + 2 * c, ld)) = make_float2((float)o[0], (float)o[1]);
-    }
-  }
-}
-
-template <int NT, typename T, bool MUON>
-__global__ void __launch_bounds__(kThreads) ortho_kernel(const __grid_constant__ Args a) {
-  using D_ = Dims<NT>;
-  extern __shared__ __align__(16) double sm[];
-  double *G = sm, *work = sm + D_::MAT, *part = work + D_::WORK;
-  double *S = work, *P = work + D_::MAT, *V = work + 2 * D_::MAT;
-  float* x = reinterpret_cast<float*>(part + D_::PART);
-  const int warp = threadIdx.x >> 5;
-  const int rank = blockIdx.x % a.cluster, ld = a.cap + 8;
-  const long long mat = blockIdx.x / a.cluster;
-  int ti = 0;
-  while (ti + 1 < a.n && a.t[ti + 1].start <= mat) ++ti;
-  const Tensor& t = a.t[ti];
-  const long long base = (mat - t.start) * (long long)t.d * t.L;
-  const int slice = ((t.L + a.cluster - 1) / a.cluster + 7) & ~7;
-  const int s0 = min(rank * slice, t.L), s1 = min(s0 + slice, t.L);
-  const int chunks = (s1 - s0 + a.cap - 1) / a.cap;
-
-  const int grp = warp % D_::GROUPS, kg = warp / D_::GROUPS;
-  double acc[D_::TILES][2];
-#pragma unroll
-  for (int n = 0; n < D_::TILES; ++n) acc[n][0] = acc[n][1] = 0.0;
-  for (int ch = 0; ch < chunks; ++ch) {
-    const int j0 = s0 + ch * a.cap, w = min(a.cap, s1 - j0);
-    if (ch) __syncthreads();
-    load_slice<T, MUON>(a, t, base, j0, w, x, ld, D_::D, true);
-    __syncthreads();
+__device__ __forceinline__ void gram_group(int grp, const float* x, int ld, int w, int kg,
+                                           double (&acc)[Dims<NT>::ACC][2]) {
+  if constexpr (Dims<NT>::GROUPS == 1) {
+    gram<NT, 0>(x, ld, w, kg, acc);
+  } else {
     switch (grp) {
       case 0: gram<NT, 0>(x, ld, w, kg, acc); break;
       case 1: gram<NT, 1>(x, ld, w, kg, acc); break;
@@ -337,23 +382,34 @@ __global__ void __launch_bounds__(kThreads) ortho_kernel(const __grid_constant__
       default: gram<NT, 3>(x, ld, w, kg, acc); break;
     }
   }
-  // the warps' partial sums, halved until BUFS are left, then added in order
-  auto pack_group = [&](double* dst, bool add) {
+}
+template <int NT, bool ADD>
+__device__ __forceinline__ void pack_group(int grp, double* part, double (&acc)[Dims<NT>::ACC][2]) {
+  if constexpr (Dims<NT>::GROUPS == 1) {
+    pack<NT, 0, ADD>(part, acc);
+  } else {
     switch (grp) {
-      case 0: add ? pack<NT, 0, true>(dst, acc) : pack<NT, 0, false>(dst, acc); break;
-      case 1: add ? pack<NT, 1, true>(dst, acc) : pack<NT, 1, false>(dst, acc); break;
-      case 2: add ? pack<NT, 2, true>(dst, acc) : pack<NT, 2, false>(dst, acc); break;
-      default: add ? pack<NT, 3, true>(dst, acc) : pack<NT, 3, false>(dst, acc); break;
+      case 0: pack<NT, 0, ADD>(part, acc); break;
+      case 1: pack<NT, 1, ADD>(part, acc); break;
+      case 2: pack<NT, 2, ADD>(part, acc); break;
+      default: pack<NT, 3, ADD>(part, acc); break;
     }
-  };
+  }
+}
+
+// The warps' partial Gram matrices into `part`: halved until BUFS are left, then added in order. `work`: BUFS parts.
+template <int NT>
+__device__ __forceinline__ void reduce_warps(double (&acc)[Dims<NT>::ACC][2], double* work, double* part) {
+  using D_ = Dims<NT>;
+  const int warp = threadIdx.x >> 5, grp = warp % D_::GROUPS, kg = warp / D_::GROUPS;
 #pragma unroll
   for (int h = D_::KG; h > D_::BUFS; h /= 2) {
-    if (kg >= h / 2 && kg < h) pack_group(work + (kg - h / 2) * D_::PART, false);
+    if (kg >= h / 2 && kg < h) pack_group<NT, false>(grp, work + (kg - h / 2) * D_::PART, acc);
     __syncthreads();
-    if (kg < h / 2) pack_group(work + kg * D_::PART, true);
+    if (kg < h / 2) pack_group<NT, true>(grp, work + kg * D_::PART, acc);
     __syncthreads();
   }
-  if (kg < D_::BUFS) pack_group(work + kg * D_::PART, false);
+  if (kg < D_::BUFS) pack_group<NT, false>(grp, work + kg * D_::PART, acc);
   __syncthreads();
   for (int q = threadIdx.x; q < D_::PART; q += kThreads) {
     double s = work[q];
@@ -361,100 +417,477 @@ __global__ void __launch_bounds__(kThreads) ortho_kernel(const __grid_constant__
     for (int b = 1; b < D_::BUFS; ++b) s += work[b * D_::PART + q];
     part[q] = s;
   }
-  if (a.cluster > 1) {
-    cluster_arrive();
-    cluster_wait();
-  } else {
-    __syncthreads();
-  }
-  for (int q = threadIdx.x; q < D_::PART; q += kThreads) {
-    double s = 0.0;
-    if (a.cluster > 1)
-      for (int r = 0; r < a.cluster; ++r) s += ld_cluster(part + q, r);
-    else
-      s = part[q];
-    int i, j;
-    tile_of<NT>(q >> 6, i, j);
-    const int r = 8 * i + ((q & 63) >> 3), k = 8 * j + (q & 7);
-    G[r * D_::LDM + k] = s;
-    if (i != j) G[k * D_::LDM + r] = s;
-  }
-  if (a.cluster > 1) cluster_arrive();  // this block has read the others' parts
-  __syncthreads();
-  iterate<NT>(a, G, S, P, V);
-  for (int ch = chunks - 1; ch >= 0; --ch) {  // the last chunk is still there
-    const int j0 = s0 + ch * a.cap, w = min(a.cap, s1 - j0);
-    if (ch < chunks - 1) {
-      __syncthreads();
-      load_slice<T, MUON>(a, t, base, j0, w, x, ld, D_::D, false);
-      __syncthreads();
-    }
-    apply<NT>(P, x, ld, w);
-    __syncthreads();
-    store_slice<T, MUON>(a, t, base, j0, w, x, ld);
-  }
-  if (a.cluster > 1) cluster_wait();  // its part stays until every block has read it
 }
 
-constexpr int kSmemMax = 227 * 1024;
-
-// Columns of x that a block of NT row tiles can hold.
+// Tile n of the upper triangle.
 template <int NT>
-constexpr int max_cols() {
-  return (int)((kSmemMax - Dims<NT>::kFixed) / (NT * 8 * 4) - 8) / 32 * 32;
+__device__ __forceinline__ void tile_of(int n, int& i, int& j) {
+  i = 0;
+#pragma unroll
+  for (int k = 1; k < NT; ++k)
+    if (n >= tri<NT>(k, k)) i = k;
+  j = n - tri<NT>(i, i) + i;
+}
+
+// Element q of the packed upper triangle to both its places.
+template <int NT>
+__device__ __forceinline__ void spread(double* M, int q, double v) {
+  int i, j;
+  tile_of<NT>(q >> 6, i, j);
+  M[(i * NT + j) * 64 + (q & 63)] = v;
+  if (i != j) M[(j * NT + i) * 64 + (q & 7) * 8 + ((q >> 3) & 7)] = v;
+}
+
+// c = tile (i, j) of A B.
+template <int NT>
+__device__ __forceinline__ void product(const double* A, const double* B, int i, int j, double (&c)[2]) {
+  const int lane = threadIdx.x & 31;
+  const double2* pa = reinterpret_cast<const double2*>(A + i * NT * 64) + lane;
+  const double2* pb = reinterpret_cast<const double2*>(B + j * NT * 64) + lane;
+  double c1[2] = {0.0, 0.0};
+  c[0] = c[1] = 0.0;
+#pragma unroll
+  for (int k = 0; k < NT; ++k) {
+    const double2 a = pa[32 * k], b = pb[32 * k];
+    dmma(c, a.x, b.x);
+    dmma(c1, a.y, b.y);
+  }
+  c[0] += c1[0];
+  c[1] += c1[1];
+}
+
+// Writes a tile and its mirror image.
+template <int NT>
+__device__ __forceinline__ void put_tile(double* M, int i, int j, const double (&c)[2]) {
+  const int lane = threadIdx.x & 31;
+  *reinterpret_cast<double2*>(M + (i * NT + j) * 64 + 2 * lane) = make_double2(c[0], c[1]);
+  if (i != j) {
+    double* m = M + (j * NT + i) * 64 + (lane & 3) * 16 + (lane >> 2);
+    m[0] = c[0];
+    m[8] = c[1];
+  }
+}
+
+// From the Gram matrix G of x (unscaled) to P with P x = the polynomial of x, in M[0] or M[1] (returned through P). work
+// holds S, V, M[0], M[1]. Returns whether no entry of P / inv (the polynomial's own matrix) is above kMaxPlain: the
+// product with x may then be fp32, whose d roundings stay near 2^-22 of the result. Gradients of low rank have entries
+// up to 485, and the sum cancels them.
+constexpr double kMaxPlain = 8.0;
+template <int NT>
+__device__ bool iterate(const Args& a, double* G, double* work, double*& P) {
+  using D_ = Dims<NT>;
+  double *S = work, *V = work + D_::MAT, *M = work + 2 * D_::MAT;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  double tr = 0.0;
+  for (int i = lane; i < D_::D; i += 32) tr += G[(i >> 3) * (NT + 1) * 64 + (i & 7) * 9];
+#pragma unroll
+  for (int o = 16; o; o >>= 1) tr += __shfl_xor_sync(0xffffffffu, tr, o);
+  const double inv = 1.0 / (sqrt(tr) + a.eps);
+  double sc = inv * inv;  // the first step's G still has to be scaled by it
+  for (int step = 0; step < a.steps; ++step) {
+    const double ca = a.coef[step][0], cb = a.coef[step][1] * sc, cc = a.coef[step][2] * sc * sc;
+    const bool last = step + 1 == a.steps;
+    double *from = M + ((step + 1) & 1) * D_::MAT, *to = M + (step & 1) * D_::MAT;
+    for (int n = warp; n < D_::TILES; n += kWarps) {
+      int i, j;
+      tile_of<NT>(n, i, j);
+      const double2 g = *reinterpret_cast<const double2*>(G + (i * NT + j) * 64 + 2 * lane);
+      double c[2];
+      product<NT>(G, G, i, j, c);
+      const int r = lane >> 2, k = 2 * (lane & 3);
+      c[0] = cb * g.x + cc * c[0] + (i == j && r == k ? ca : 0.0);
+      c[1] = cb * g.y + cc * c[1] + (i == j && r == k + 1 ? ca : 0.0);
+      put_tile<NT>(S, i, j, c);
+      if (step == 0) put_tile<NT>(to, i, j, c);
+    }
+    __syncthreads();
+    // P' = S P (from the second step on) and V = S G (but in the last), each tile by its own warp
+    const int np = step ? D_::TILES : 0, nv = last ? 0 : D_::TILES;
+    for (int n = warp; n < np + nv; n += kWarps) {
+      const bool isp = n < np;
+      int i, j;
+      tile_of<NT>(isp ? n : n - np, i, j);
+      double c[2];
+      product<NT>(S, isp ? from : G, i, j, c);
+      put_tile<NT>(isp ? to : V, i, j, c);
+    }
+    if (last) break;
+    __syncthreads();
+    for (int n = warp; n < D_::TILES; n += kWarps) {
+      int i, j;
+      tile_of<NT>(n, i, j);
+      double c[2];
+      product<NT>(S, V, i, j, c);
+      c[0] *= sc;
+      c[1] *= sc;
+      put_tile<NT>(G, i, j, c);
+    }
+    __syncthreads();
+    sc = 1.0;
+  }
+  __syncthreads();
+  P = M + ((a.steps - 1) & 1) * D_::MAT;
+  // the scale itself has to be a normal fp32 number with room for the sums
+  bool plain = inv > 1e-30 && inv < 1e30;
+  for (int q = threadIdx.x; q < D_::MAT; q += kThreads) {
+    plain = plain && fabs(P[q]) <= kMaxPlain;  // false for NaN
+    P[q] *= inv;
+  }
+  return __syncthreads_and(plain);
+}
+
+// P's fp32 copy, row k then column i.
+template <int NT>
+__device__ __forceinline__ void round_form(const double* P, float* Pf) {
+  for (int q = threadIdx.x; q < Dims<NT>::MAT; q += kThreads) {
+    const int tile = q >> 6, i = (tile / NT) * 8 + ((q >> 3) & 7), k = (tile % NT) * 8 + (q & 7);
+    Pf[k * NT * 8 + i] = (float)P[q];
+  }
+}
+
+// x <- P x in place in fp64: a warp owns eight columns at a time.
+template <int NT>
+__device__ __forceinline__ void apply(const double* P, float* x, int ld, int w) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+  const double2* p = reinterpret_cast<const double2*>(P) + lane;
+  for (int j = warp * 8; j < w; j += kWarps * 8) {
+    double o[NT][2];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = 0.0;
+    const float* b = x + 2 * c * ld + j + r;
+#pragma unroll
+    for (int k = 0; k < NT; ++k) {
+      const double b0 = b[8 * k * ld], b1 = b[(8 * k + 1) * ld];
+      double2 f[NT];
+#pragma unroll
+      for (int i = 0; i < NT; ++i) f[i] = p[(i * NT + k) * 32];
+#pragma unroll
+      for (int i = 0; i < NT; ++i) dmma(o[i], f[i].x, b0);
+#pragma unroll
+      for (int i = 0; i < NT; ++i) dmma(o[i], f[i].y, b1);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+      *reinterpret_cast<float2*>(x + (8 * i + r) * ld + j + 2 * c) = make_float2((float)o[i][0], (float)o[i][1]);
+  }
+}
+
+// The same in fp32: a thread owns two columns, and reads row k of P as a broadcast.
+template <int NT>
+__device__ __forceinline__ void apply_plain(const float* Pf, float* x, int ld, int w) {
+  constexpr int D = NT * 8;
+  for (int j = threadIdx.x * 2; j < w; j += kThreads * 2) {
+    float o[D][2];
+#pragma unroll
+    for (int i = 0; i < D; ++i) o[i][0] = o[i][1] = 0.f;
+#pragma unroll 4
+    for (int k = 0; k < D; ++k) {
+      const float2 v = *reinterpret_cast<const float2*>(x + k * ld + j);
+#pragma unroll
+      for (int i = 0; i < D; i += 4) {
+        const float4 p = *reinterpret_cast<const float4*>(Pf + k * D + i);
+        o[i][0] = fmaf(p.x, v.x, o[i][0]);
+        o[i][1] = fmaf(p.x, v.y, o[i][1]);
+        o[i + 1][0] = fmaf(p.y, v.x, o[i + 1][0]);
+        o[i + 1][1] = fmaf(p.y, v.y, o[i + 1][1]);
+        o[i + 2][0] = fmaf(p.z, v.x, o[i + 2][0]);
+        o[i + 2][1] = fmaf(p.z, v.y, o[i + 2][1]);
+        o[i + 3][0] = fmaf(p.w, v.x, o[i + 3][0]);
+        o[i + 3][1] = fmaf(p.w, v.y, o[i + 3][1]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < D; ++i) *reinterpret_cast<float2*>(x + i * ld + j) = make_float2(o[i][0], o[i][1]);
+  }
+}
+
+// The tensor of matrix `mat` and its first element.
+__device__ __forceinline__ const Tensor& tensor_of(const Args& a, long long mat, long long& base) {
+  int ti = 0;
+  for (int end = a.n; end - ti > 1;) {
+    const int mid = (ti + end) / 2;
+    if (a.t[mid].start <= mat) ti = mid;
+    else end = mid;
+  }
+  base = (mat - a.t[ti].start) * (long long)a.t[ti].d * a.t[ti].L;
+  return a.t[ti];
+}
+
+// Resident: the blocks of a cluster hold one matrix, `cap` columns each at most.
+template <int NT, typename T, bool MUON>
+__global__ void __launch_bounds__(kThreads, NT <= 2 ? 4 : 2) ortho_kernel(const __grid_constant__ Args a) {
+  using D_ = Dims<NT>;
+  extern __shared__ __align__(16) double sm[];
+  double *G = sm, *part = G + D_::MAT, *work = part + D_::PART;
+  float* x = reinterpret_cast<float*>(work + D_::WORK);
+  const int rank = blockIdx.x % a.blocks, ld = pitch(a.cap);
+  long long base;
+  const Tensor& t = tensor_of(a, blockIdx.x / a.blocks, base);
+  const int slice = ((t.L + a.blocks - 1) / a.blocks + 7) & ~7;
+  const int j0 = min(rank * slice, t.L), w = min(slice, t.L - j0);
+
+  double acc[D_::ACC][2];
+#pragma unroll
+  for (int n = 0; n < D_::ACC; ++n) acc[n][0] = acc[n][1] = 0.0;
+  if (w) load_slice<NT, T, MUON>(a, t, base, j0, w, x, ld, true);
+  __syncthreads();
+  gram<NT, 0>(x, ld, w, threadIdx.x >> 5, acc);
+  reduce_warps<NT>(acc, work, part);
+  if (a.blocks > 1) {
+    cluster_arrive();
+    cluster_wait();
+    for (int q = threadIdx.x; q < D_::PART; q += kThreads) {
+      double v[8], s = 0.0;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) v[r] = r < a.blocks ? ld_cluster(part + q, r) : 0.0;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) s += v[r];
+      spread<NT>(G, q, s);
+    }
+    cluster_arrive();  // this block has read the others' parts
+  } else {
+    __syncthreads();
+    for (int q = threadIdx.x; q < D_::PART; q += kThreads) spread<NT>(G, q, part[q]);
+  }
+  __syncthreads();
+  double* P;
+  if (iterate<NT>(a, G, work, P)) {
+    float* Pf = reinterpret_cast<float*>(G);
+    round_form<NT>(P, Pf);
+    __syncthreads();
+    apply_plain<NT>(Pf, x, ld, w);
+  } else {
+    apply<NT>(P, x, ld, w);
+  }
+  __syncthreads();
+  if (w) store_slice<T, MUON>(a, t, base, j0, w, x, ld);
+  if (a.blocks > 1) cluster_wait();  // its part stays until every block has read it
+}
+
+// Split: block b of a matrix takes the chunks b, b + blocks, ... of `cap` columns.
+template <int NT, typename T, bool MUON>
+__global__ void __launch_bounds__(kThreads, 2) gram_kernel(const __grid_constant__ Args a) {
+  using D_ = Dims<NT>;
+  extern __shared__ __align__(16) double sm[];
+  double* work = sm;
+  float* x = reinterpret_cast<float*>(work + D_::BUFS * D_::PART);
+  const int block = blockIdx.x % a.blocks, ld = pitch(a.cap), warp = threadIdx.x >> 5;
+  long long base;
+  const Tensor& t = tensor_of(a, blockIdx.x / a.blocks, base);
+  double acc[D_::ACC][2];
+#pragma unroll
+  for (int n = 0; n < D_::ACC; ++n) acc[n][0] = acc[n][1] = 0.0;
+  for (int j0 = block * a.cap; j0 < t.L; j0 += a.blocks * a.cap) {
+    const int w = min(a.cap, t.L - j0);
+    load_slice<NT, T, MUON>(a, t, base, j0, w, x, ld, true);
+    __syncthreads();
+    gram_group<NT>(warp % D_::GROUPS, x, ld, w, warp / D_::GROUPS, acc);
+    __syncthreads();
+  }
+  reduce_warps<NT>(acc, work, a.gram + (long long)blockIdx.x * D_::PART);
+}
+
+// One block per matrix: the parts in order, then P.
+template <int NT>
+__global__ void __launch_bounds__(kThreads) form_kernel(const __grid_constant__ Args a) {
+  using D_ = Dims<NT>;
+  extern __shared__ __align__(16) double sm[];
+  double *G = sm, *work = G + D_::MAT;
+  const double* part = a.gram + (long long)blockIdx.x * a.blocks * D_::PART;
+  for (int q = threadIdx.x; q < D_::PART; q += kThreads) {
+    double s = 0.0;
+#pragma unroll 8
+    for (int b = 0; b < a.blocks; ++b) s += part[(long long)b * D_::PART + q];
+    spread<NT>(G, q, s);
+  }
+  __syncthreads();
+  double* P;
+  const bool plain = iterate<NT>(a, G, work, P);
+  double* out = a.form + (long long)blockIdx.x * (D_::MAT + 2);
+  for (int q = threadIdx.x; q < D_::MAT; q += kThreads) out[q] = P[q];
+  if (threadIdx.x == 0) out[D_::MAT] = plain ? 1.0 : 0.0;
 }
 
 template <int NT, typename T, bool MUON>
-int launch(Args& a, long long matrices, int maxL, cudaStream_t st) {
-  int c = 1;
-  while (c < 8 && maxL > 256 * c) c *= 2;
-  const int slice = ((maxL + c - 1) / c + 31) / 32 * 32;
-  a.cluster = c;
-  a.cap = std::min(slice, max_cols<NT>());
-  const long long smem = Dims<NT>::kFixed + (long long)NT * 8 * (a.cap + 8) * 4;
-  SMELB_CHECK_ARG(matrices * c < (1LL << 31), kErrShape, "orthogonalize: %lld matrices", matrices);
-  auto kern = ortho_kernel<NT, T, MUON>;
+__global__ void __launch_bounds__(kThreads) product_kernel(const __grid_constant__ Args a) {
+  using D_ = Dims<NT>;
+  extern __shared__ __align__(16) double sm[];
+  float* x = reinterpret_cast<float*>(sm + D_::MAT);
+  const int block = blockIdx.x % a.blocks, ld = pitch(a.cap);
+  const long long mat = blockIdx.x / a.blocks;
+  long long base;
+  const Tensor& t = tensor_of(a, mat, base);
+  const double* form = a.form + mat * (D_::MAT + 2);
+  const bool plain = form[D_::MAT] != 0.0;
+  if (plain) round_form<NT>(form, reinterpret_cast<float*>(sm));
+  else
+    for (int q = threadIdx.x; q < D_::MAT; q += kThreads) sm[q] = form[q];
+  for (int j0 = block * a.cap; j0 < t.L; j0 += a.blocks * a.cap) {
+    const int w = min(a.cap, t.L - j0);
+    load_slice<NT, T, MUON>(a, t, base, j0, w, x, ld, false);
+    __syncthreads();
+    if (plain) apply_plain<NT>(reinterpret_cast<float*>(sm), x, ld, w);
+    else apply<NT>(sm, x, ld, w);
+    __syncthreads();
+    store_slice<T, MUON>(a, t, base, j0, w, x, ld);
+    __syncthreads();
+  }
+}
+
+void set_cap(Args& a, int cap) {
+  a.cap = cap;
+  a.by_v[0] = (uint32_t)((1ull << 32) / (cap / 4) + 1);
+  a.by_v[1] = (uint32_t)((1ull << 32) / (cap / 8) + 1);
+}
+
+template <typename F>
+int launch(F* kern, const Args& a, long long blocks, long long smem, int cluster, cudaStream_t st) {
+  SMELB_CHECK_ARG(blocks < (1LL << 31), kErrShape, "orthogonalize: %lld blocks", blocks);
   SMELB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(matrices * c));
+  cfg.gridDim = dim3((unsigned)blocks);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim = {(unsigned)c, 1, 1};
+  at[0].val.clusterDim = {(unsigned)cluster, 1, 1};
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 1 ? 1 : 0;
   SMELB_CUDA(cudaLaunchKernelEx(&cfg, kern, a));
   count_launch();
   return kOk;
 }
 
-template <int NT>
-int launch_typed(Args& a, bool bf, bool muon, long long matrices, int maxL, cudaStream_t st) {
-  if (muon) return bf ? launch<NT, bf16, true>(a, matrices, maxL, st) : launch<NT, float, true>(a, matrices, maxL, st);
-  return bf ? launch<NT, bf16, false>(a, matrices, maxL, st) : launch<NT, float, false>(a, matrices, maxL, st);
+// Columns of a resident block at most: 45 KB for 16 rows (four blocks to an SM; 1024 columns in two ran 7% slower on 1548
+// matrices of 16 x 512 .. 2048), 112 KB for 32 (two blocks).
+constexpr int kBlockCols = 512, kMaxBlocks = 8;
+
+// Whether matrices of this size are held by a cluster: up to 32 rows, and no more columns than eight blocks hold.
+bool resident(int nt, int L) { return nt <= 4 && L <= kBlockCols * kMaxBlocks; }
+
+constexpr int kSplitCap = 128;
+
+// Blocks for one matrix of the split way.
+int split_blocks(long long matrices, int L) {
+  const long long chunks = (L + kSplitCap - 1) / kSplitCap;
+  const long long want = (148 * 4 + matrices - 1) / matrices;  // four blocks to an SM
+  return (int)std::max<long long>(1, std::min<long long>(chunks, std::min<long long>(want, 296)));
 }
 
-// Row tiles that the kernel is built for.
+template <int NT, typename T, bool MUON>
+int run_resident(Args& a, long long matrices, int maxL, cudaStream_t st) {
+  using D_ = Dims<NT>;
+  int c = 1;
+  while (c < kMaxBlocks && (maxL > kBlockCols * c || (maxL > 256 * c && matrices * c < 296))) c *= 2;
+  a.blocks = c;
+  set_cap(a, ((maxL + c - 1) / c + 31) / 32 * 32);
+  const long long smem = (long long)(D_::MAT + D_::PART + D_::WORK) * 8 + (long long)NT * 8 * pitch(a.cap) * 4;
+  return launch(ortho_kernel<NT, T, MUON>, a, matrices * c, smem, c, st);
+}
+
+template <int NT, typename T, bool MUON>
+int run_split(Args& a, long long matrices, int maxL, double* ws, cudaStream_t st) {
+  using D_ = Dims<NT>;
+  a.blocks = split_blocks(matrices, maxL);
+  set_cap(a, kSplitCap);
+  a.gram = ws;
+  a.form = ws + matrices * a.blocks * D_::PART;
+  const long long x = (long long)NT * 8 * pitch(a.cap) * 4;
+  int rc = launch(gram_kernel<NT, T, MUON>, a, matrices * a.blocks, (long long)D_::BUFS * D_::PART * 8 + x, 1, st);
+  if (rc == kOk) rc = launch(form_kernel<NT>, a, matrices, (long long)(D_::MAT + D_::WORK) * 8, 1, st);
+  if (rc == kOk) rc = launch(product_kernel<NT, T, MUON>, a, matrices * a.blocks, (long long)D_::MAT * 8 + x, 1, st);
+  return rc;
+}
+
+template <int NT, typename T, bool MUON>
+int run_way(Args& a, long long matrices, int maxL, bool held, double* ws, cudaStream_t st) {
+  if constexpr (NT <= 4)
+    if (held) return run_resident<NT, T, MUON>(a, matrices, maxL, st);
+  return run_split<NT, T, MUON>(a, matrices, maxL, ws, st);
+}
+
+template <int NT>
+int run_typed(Args& a, bool bf, bool muon, long long matrices, int maxL, bool held, double* ws, cudaStream_t st) {
+  if (muon)
+    return bf ? run_way<NT, bf16, true>(a, matrices, maxL, held, ws, st)
+              : run_way<NT, float, true>(a, matrices, maxL, held, ws, st);
+  return bf ? run_way<NT, bf16, false>(a, matrices, maxL, held, ws, st)
+            : run_way<NT, float, false>(a, matrices, maxL, held, ws, st);
+}
+
+// Row tiles that the kernels are built for.
 int tiles_for(int d) {
   const int n = (d + 7) / 8;
   return n <= 4 ? n : n <= 6 ? 6 : 8;
 }
+constexpr int kTileCounts[] = {1, 2, 3, 4, 6, 8};
+
+int check_shapes(const smelb_muon_tensor* t, int64_t n, const char* what) {
+  SMELB_CHECK_ARG(t || n == 0, kErrArg, "%s: null pointer", what);
+  for (int64_t i = 0; i < n; ++i) {
+    SMELB_CHECK_ARG(t[i].batch >= 0 && t[i].rows >= 1 && t[i].cols >= 1 && std::min(t[i].rows, t[i].cols) <= kMaxD &&
+                        std::max(t[i].rows, t[i].cols) < (1LL << 24) && t[i].batch < (1LL << 28),
+                    kErrShape, "%s: tensor %lld: %lld x %lld x %lld (short side 1..%d)", what, (long long)i,
+                    (long long)t[i].batch, (long long)t[i].rows, (long long)t[i].cols, kMaxD);
+  }
+  return kOk;
+}
+
+// Calls f(row tiles, held, first tensor.., matrices, longest side) for every launch: tensors of the same row tiles and the
+// same way, at most kMaxTensors. The list of a launch is idx[0 .. count).
+template <typename F>
+int for_launches(const smelb_muon_tensor* t, int64_t n, F&& f) {
+  for (int nt : kTileCounts)
+    for (int held = 0; held < 2; ++held) {
+      int64_t idx[kMaxTensors];
+      int count = 0, maxL = 0;
+      long long matrices = 0;
+      for (int64_t i = 0; i < n; ++i) {
+        const int d = (int)std::min(t[i].rows, t[i].cols), L = (int)std::max(t[i].rows, t[i].cols);
+        if (t[i].batch == 0 || tiles_for(d) != nt || resident(nt, L) != (held != 0)) continue;
+        idx[count++] = i;
+        matrices += t[i].batch;
+        maxL = std::max(maxL, L);
+        if (count == kMaxTensors) {
+          if (int rc = f(nt, held != 0, idx, count, matrices, maxL)) return rc;
+          count = maxL = 0;
+          matrices = 0;
+        }
+      }
+      if (count)
+        if (int rc = f(nt, held != 0, idx, count, matrices, maxL)) return rc;
+    }
+  return kOk;
+}
+
+// Bytes that the split launches of a call need, the largest of them (a launch reuses the one before's).
+long long workspace(const smelb_muon_tensor* t, int64_t n) {
+  long long most = 0;
+  for_launches(t, n, [&](int nt, bool held, const int64_t*, int, long long matrices, int maxL) {
+    if (!held) {
+      const long long part = nt * (nt + 1) / 2 * 64, form = nt * nt * 64 + 2;
+      most = std::max(most, matrices * (split_blocks(matrices, maxL) * part + form) * 8);
+    }
+    return 0;
+  });
+  return most;
+}
 
 int run(const smelb_muon_tensor* t, int64_t n, int dtype, bool muon, double lr, double mu, bool nesterov, double wd,
-        int adjust, int steps, const double* coef, double eps, const char* what, cudaStream_t st) {
-  SMELB_CHECK_ARG(t || n == 0, kErrArg, "%s: null pointer", what);
+        int adjust, int steps, const double* coef, double eps, void* ws, int64_t ws_bytes, const char* what,
+        cudaStream_t st) {
+  if (int rc = check_shapes(t, n, what)) return rc;
+  for (int64_t i = 0; i < n; ++i)
+    SMELB_CHECK_ARG(t[i].batch == 0 || (t[i].p && t[i].g && (t[i].m || !muon)), kErrArg, "%s: null pointer", what);
   SMELB_CHECK_ARG(dtype == 0 || dtype == 1, kErrDtype, "%s: dtype %d", what, dtype);
   SMELB_CHECK_ARG(steps >= 1 && steps <= kMaxSteps && coef, kErrArg, "%s: %d steps (1..%d)", what, steps, kMaxSteps);
   SMELB_CHECK_ARG(eps > 0.0, kErrArg, "%s: eps must be positive", what);
-  for (int64_t i = 0; i < n; ++i) {
-    SMELB_CHECK_ARG(t[i].batch >= 0 && t[i].rows >= 1 && t[i].cols >= 1 && std::min(t[i].rows, t[i].cols) <= kMaxD &&
-                        std::max(t[i].rows, t[i].cols) < (1LL << 24) && t[i].batch < (1LL << 31),
-                    kErrShape, "%s: tensor %lld: %lld x %lld x %lld (short side 1..%d)", what, (long long)i,
-                    (long long)t[i].batch, (long long)t[i].rows, (long long)t[i].cols, kMaxD);
-    SMELB_CHECK_ARG(t[i].batch == 0 || (t[i].p && t[i].g && (t[i].m || !muon)), kErrArg, "%s: null pointer", what);
-  }
+  const long long need = workspace(t, n);
+  SMELB_CHECK_ARG(ws_bytes >= need && (ws || !need), kErrWorkspace, "%s: workspace %lld bytes, %lld needed", what,
+                  (long long)ws_bytes, need);
+  SMELB_CHECK_ARG(((uintptr_t)ws & 255) == 0, kErrArg, "%s: workspace must be 256-byte aligned", what);
   Args a{};
   a.steps = steps;
   a.mu = (float)mu;
@@ -464,38 +897,29 @@ int run(const smelb_muon_tensor* t, int64_t n, int dtype, bool muon, double lr, 
   a.eps = eps;
   for (int s = 0; s < steps; ++s)
     for (int k = 0; k < 3; ++k) a.coef[s][k] = coef[3 * s + k];
-  for (int nt : {1, 2, 3, 4, 6, 8}) {
-    long long matrices = 0;
-    int maxL = 0;
-    a.n = 0;
-    auto flush = [&]() -> int {
-      if (!a.n) return kOk;
-      const bool bf = dtype == 1;
-      const int rc = nt == 1   ? launch_typed<1>(a, bf, muon, matrices, maxL, st)
-                     : nt == 2 ? launch_typed<2>(a, bf, muon, matrices, maxL, st)
-                     : nt == 3 ? launch_typed<3>(a, bf, muon, matrices, maxL, st)
-                     : nt == 4 ? launch_typed<4>(a, bf, muon, matrices, maxL, st)
-                     : nt == 6 ? launch_typed<6>(a, bf, muon, matrices, maxL, st)
-                               : launch_typed<8>(a, bf, muon, matrices, maxL, st);
-      a.n = 0;
-      matrices = 0;
-      maxL = 0;
-      return rc;
-    };
-    for (int64_t i = 0; i < n; ++i) {
-      const int d = (int)std::min(t[i].rows, t[i].cols), L = (int)std::max(t[i].rows, t[i].cols);
-      if (t[i].batch == 0 || tiles_for(d) != nt) continue;
-      const double ratio = (double)t[i].rows / (double)t[i].cols;
-      const double f = adjust == 1 ? 0.2 * sqrt((double)L) : sqrt(std::max(1.0, ratio));
-      a.t[a.n++] = Tensor{t[i].p, t[i].g, t[i].m, matrices, d, L, t[i].rows > t[i].cols ? 1 : 0, (float)(lr * f)};
-      matrices += t[i].batch;
-      maxL = std::max(maxL, L);
-      if (a.n == kMaxTensors)
-        if (int rc = flush()) return rc;
+  return for_launches(t, n, [&](int nt, bool held, const int64_t* idx, int count, long long matrices, int maxL) {
+    a.n = count;
+    long long start = 0;
+    for (int k = 0; k < count; ++k) {
+      const smelb_muon_tensor& s = t[idx[k]];
+      const int d = (int)std::min(s.rows, s.cols), L = (int)std::max(s.rows, s.cols);
+      const double f = adjust == 1 ? 0.2 * sqrt((double)L) : sqrt(std::max(1.0, (double)s.rows / (double)s.cols));
+      // a single column is a single row in memory
+      a.t[k] = Tensor{s.p, s.g, s.m, start, d, L, s.rows > s.cols && d > 1 ? 1 : 0, (uint32_t)((1ull << 32) / d + 1),
+                      (float)(lr * f)};
+      start += s.batch;
     }
-    if (int rc = flush()) return rc;
-  }
-  return kOk;
+    const bool bf = dtype == 1;
+    double* w = (double*)ws;
+    switch (nt) {
+      case 1: return run_typed<1>(a, bf, muon, matrices, maxL, held, w, st);
+      case 2: return run_typed<2>(a, bf, muon, matrices, maxL, held, w, st);
+      case 3: return run_typed<3>(a, bf, muon, matrices, maxL, held, w, st);
+      case 4: return run_typed<4>(a, bf, muon, matrices, maxL, held, w, st);
+      case 6: return run_typed<6>(a, bf, muon, matrices, maxL, held, w, st);
+      default: return run_typed<8>(a, bf, muon, matrices, maxL, held, w, st);
+    }
+  });
 }
 
 }  // namespace
@@ -505,18 +929,30 @@ using namespace smelb;
 
 extern "C" {
 
+int64_t smelb_muon_workspace_bytes(const smelb_muon_tensor* tensors, int64_t n) {
+  if (n < 0 || check_shapes(tensors, n, "muon_workspace_bytes") != kOk) return -1;
+  return workspace(tensors, n);
+}
+
+int64_t smelb_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols) {
+  const smelb_muon_tensor t{nullptr, nullptr, nullptr, batch, rows, cols};
+  return smelb_muon_workspace_bytes(&t, 1);
+}
+
 int smelb_orthogonalize(const void* x, int dtype, int64_t batch, int64_t rows, int64_t cols, int steps,
-                        const double* coefficients, double eps, void* out, void* stream) {
+                        const double* coefficients, double eps, void* out, void* workspace, int64_t workspace_bytes,
+                        void* stream) {
   const smelb_muon_tensor t{out, x, nullptr, batch, rows, cols};
-  return run(&t, 1, dtype, false, 0.0, 0.0, false, 0.0, 0, steps, coefficients, eps, "orthogonalize",
-             (cudaStream_t)stream);
+  return run(&t, 1, dtype, false, 0.0, 0.0, false, 0.0, 0, steps, coefficients, eps, workspace, workspace_bytes,
+             "orthogonalize", (cudaStream_t)stream);
 }
 
 int smelb_muon_step(const smelb_muon_tensor* tensors, int64_t n, int dtype, double lr, double momentum, int nesterov,
-                    double weight_decay, int adjust, int steps, const double* coefficients, double eps, void* stream) {
+                    double weight_decay, int adjust, int steps, const double* coefficients, double eps, void* workspace,
+                    int64_t workspace_bytes, void* stream) {
   SMELB_CHECK_ARG(n >= 0 && (adjust == 0 || adjust == 1), kErrArg, "muon_step: n=%lld adjust=%d", (long long)n, adjust);
   return run(tensors, n, dtype, true, lr, momentum, nesterov != 0, weight_decay, adjust, steps, coefficients, eps,
-             "muon_step", (cudaStream_t)stream);
+             workspace, workspace_bytes, "muon_step", (cudaStream_t)stream);
 }
 
 }  // extern "C"

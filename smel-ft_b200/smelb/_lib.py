@@ -142,9 +142,12 @@ SIGNATURES = {
     "smelb_balance_loss_bwd": (c_i32, [c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp]),
     "smelb_expert_usage": (c_i32, [c_vp, c_i64, c_vp, c_i32, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp,
                                    c_i64, c_vp]),
-    "smelb_orthogonalize": (c_i32, [c_vp, c_i32, c_i64, c_i64, c_i64, c_i32, c_vp, ctypes.c_double, c_vp, c_vp]),
+    "smelb_orthogonalize_workspace_bytes": (c_i64, [c_i64, c_i64, c_i64]),
+    "smelb_orthogonalize": (c_i32, [c_vp, c_i32, c_i64, c_i64, c_i64, c_i32, c_vp, ctypes.c_double, c_vp, c_vp, c_i64,
+                                    c_vp]),
+    "smelb_muon_workspace_bytes": (c_i64, [ctypes.POINTER(MuonTensor), c_i64]),
     "smelb_muon_step": (c_i32, [ctypes.POINTER(MuonTensor), c_i64, c_i32, ctypes.c_double, ctypes.c_double, c_i32,
-                                ctypes.c_double, c_i32, c_i32, c_vp, ctypes.c_double, c_vp]),
+                                ctypes.c_double, c_i32, c_i32, c_vp, ctypes.c_double, c_vp, c_i64, c_vp]),
     "smelb_moe_layer_size": (ctypes.c_size_t, []),
     "smelb_launch_count": (ctypes.c_longlong, []),
     "smelb_gemm_timing": (c_i32, [c_i32]),

@@ -61,8 +61,10 @@ def orthogonalize(x, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
     x = x.contiguous()
     out = torch.empty_like(x)
     if batch:
+        nb = _lib.load().smelb_orthogonalize_workspace_bytes(batch, m, n)
+        ws = torch.empty(nb, dtype=torch.uint8, device=x.device) if nb > 0 else None
         _lib.call_on(x.device, "smelb_orthogonalize", x.data_ptr(), _DTYPES[x.dtype], batch, m, n, int(steps), c,
-                     float(eps), out.data_ptr(), _lib.stream_ptr(x.device))
+                     float(eps), out.data_ptr(), _lib.ptr(ws), nb, _lib.stream_ptr(x.device))
     return out
 
 
@@ -109,8 +111,10 @@ def muon_step(params, grads, buffers, lr, momentum=0.95, nesterov=True, weight_d
             keep.append(g)
         t = table[i]
         t.p, t.g, t.m, t.batch, t.rows, t.cols = p.data_ptr(), g.data_ptr(), m.data_ptr(), batch, rows, cols
+    nb = _lib.load().smelb_muon_workspace_bytes(table, len(params))
+    ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb > 0 else None
     _lib.call_on(dev, "smelb_muon_step", table, len(params), _DTYPES[dtype], float(lr), float(momentum),
-                 1 if nesterov else 0, float(weight_decay), _ADJUST[adjust], int(steps), c, float(eps),
+                 1 if nesterov else 0, float(weight_decay), _ADJUST[adjust], int(steps), c, float(eps), _lib.ptr(ws), nb,
                  _lib.stream_ptr(dev))
 
 

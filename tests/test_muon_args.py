@@ -91,18 +91,39 @@ def test_c_entry_points_check_their_arguments():
     fake = 1 << 20  # never dereferenced: a check fails first
     coef = (ctypes.c_double * 15)(*([1.0, 0.0, 0.0] * 5))
     o = lambda **k: lib.smelb_orthogonalize(*{**dict(x=fake, dtype=0, batch=1, m=16, n=32, steps=5, coef=coef,  # noqa: E731
-                                                     eps=1e-7, out=fake, st=None), **k}.values())
+                                                     eps=1e-7, out=fake, ws=None, nb=0, st=None),
+                                                **k}.values())
     for k, rc, text in (({"x": None}, -6, "null"), ({"out": None}, -6, "null"), ({"dtype": 2}, -2, "dtype"),
                         ({"m": 0}, -1, "short side"), ({"m": 65, "n": 65}, -1, "short side"), ({"batch": -1}, -1, "-1 x"),
                         ({"n": 1 << 24}, -1, "short side"), ({"steps": 0}, -6, "steps"), ({"steps": 17}, -6, "steps"),
                         ({"coef": None}, -6, "steps"), ({"eps": 0.0}, -6, "eps"), ({"eps": float("nan")}, -6, "eps")):
         assert o(**k) == rc and text in _lib.last_error(), (k, _lib.last_error())
     assert o(batch=0, x=None, out=None) == 0
+    assert o(m=64, n=2048) == -3 and "workspace" in _lib.last_error()
+    assert o(m=64, n=2048, ws=fake + 8, nb=1 << 30) == -6 and "aligned" in _lib.last_error()
     t = (_lib.MuonTensor * 2)()
     t[0].p = t[0].g = t[0].m = fake
     t[0].batch, t[0].rows, t[0].cols = 1, 16, 32
     t[1].p = t[1].g = fake
     t[1].batch, t[1].rows, t[1].cols = 1, 16, 32
-    step = lambda n=2, adjust=0: lib.smelb_muon_step(t, n, 0, 0.1, 0.9, 1, 0.0, adjust, 5, coef, 1e-7, None)  # noqa: E731
+    step = lambda n=2, adjust=0: lib.smelb_muon_step(t, n, 0, 0.1, 0.9, 1, 0.0, adjust, 5, coef, 1e-7, None, 0,  # noqa: E731
+                                                   None)
     assert step() == -6 and "null" in _lib.last_error()  # checked for every tensor before the first launch
     assert step(adjust=2) == -6 and step(n=-1) == -6 and step(n=0) == 0
+
+
+def test_workspace_sizes():
+    """Short sides up to 32 need none unless they are longer than eight blocks hold; the rest a partial Gram matrix for each
+    block and the polynomial's matrix. The largest launch of a call decides."""
+    from smelb import _lib
+    lib = _lib.load()
+    ws = lib.smelb_orthogonalize_workspace_bytes
+    assert ws(12, 16, 2048) == 0 and ws(12, 2048, 16) == 0 and ws(5, 32, 4096) == 0 and ws(0, 64, 2048) == 0
+    assert ws(5, 32, 4097) > 0 and ws(1, 16, 4097) > 0 and ws(1, 33, 40) > 0
+    assert ws(1000, 64, 2048) >= 1000 * (36 + 64) * 64 * 8 and ws(1, 64, 1 << 20) >= 296 * 36 * 64 * 8
+    assert ws(1, 65, 65) == -1 and ws(-1, 16, 16) == -1
+    t = (_lib.MuonTensor * 2)()
+    for i, (b, m, n) in enumerate(((3, 64, 500), (7, 2000, 48))):
+        t[i].batch, t[i].rows, t[i].cols = b, m, n
+    assert lib.smelb_muon_workspace_bytes(t, 2) == max(ws(3, 64, 500), ws(7, 2000, 48))
+    assert lib.smelb_muon_workspace_bytes(t, 0) == 0 and lib.smelb_muon_workspace_bytes(None, 0) == 0
