@@ -24,6 +24,7 @@ namespace smelb {
 namespace {
 
 constexpr int kThreads = 256, kWarps = 8;
+constexpr int kSplitCap = 128;  // columns of a chunk of the split way
 constexpr int kMaxSteps = 16, kMaxTensors = 48, kMaxD = 64;
 
 struct Tensor {
@@ -333,7 +334,7 @@ template <int NT, int Q>
 __device__ __forceinline__ void gram(const float* x, int ld, int w, int kg, double (&acc)[Dims<NT>::ACC][2]) {
   const int lane = threadIdx.x & 31;
   const float* p = x + (lane >> 2) * ld + (lane & 3);
-#pragma unroll 2
+#pragma unroll (NT <= 2 ? 4 : 2)
   for (int k = kg * 4; k < w; k += Dims<NT>::KG * 4) {
     double f[NT];
 #pragma unroll
@@ -438,33 +439,85 @@ __device__ __forceinline__ void spread(double* M, int q, double v) {
   if (i != j) M[(j * NT + i) * 64 + (q & 7) * 8 + ((q >> 3) & 7)] = v;
 }
 
-// c = tile (i, j) of A B.
+// Places of an upper tile (i, j) in a matrix, for one lane: the rows of the left operand's tiles, of the right one's, the
+// tile itself and its mirror image (offsets in doubles).
 template <int NT>
-__device__ __forceinline__ void product(const double* A, const double* B, int i, int j, double (&c)[2]) {
-  const int lane = threadIdx.x & 31;
-  const double2* pa = reinterpret_cast<const double2*>(A + i * NT * 64) + lane;
-  const double2* pb = reinterpret_cast<const double2*>(B + j * NT * 64) + lane;
+struct Spot {
+  int a, b, own, mirror;
+  bool diagonal;
+  __device__ __forceinline__ explicit Spot(int n) {
+    int i, j;
+    tile_of<NT>(n, i, j);
+    set(i, j);
+  }
+  __device__ __forceinline__ Spot(int i, int j) { set(i, j); }
+  __device__ __forceinline__ void set(int i, int j) {
+    const int lane = threadIdx.x & 31;
+    a = i * NT * 64 + 2 * lane;
+    b = j * NT * 64 + 2 * lane;
+    own = (i * NT + j) * 64 + 2 * lane;
+    mirror = (j * NT + i) * 64 + (lane & 3) * 16 + (lane >> 2);
+    diagonal = i == j;
+  }
+};
+
+// c = the tile of A B.
+template <int NT>
+__device__ __forceinline__ void product(const double* A, const double* B, const Spot<NT>& t, double (&c)[2]) {
+  double2 a[NT], b[NT];
+#pragma unroll
+  for (int k = 0; k < NT; ++k) {
+    a[k] = *reinterpret_cast<const double2*>(A + t.a + 64 * k);
+    b[k] = *reinterpret_cast<const double2*>(B + t.b + 64 * k);
+  }
   double c1[2] = {0.0, 0.0};
   c[0] = c[1] = 0.0;
 #pragma unroll
   for (int k = 0; k < NT; ++k) {
-    const double2 a = pa[32 * k], b = pb[32 * k];
-    dmma(c, a.x, b.x);
-    dmma(c1, a.y, b.y);
+    dmma(c, a[k].x, b[k].x);
+    dmma(c1, a[k].y, b[k].y);
   }
   c[0] += c1[0];
   c[1] += c1[1];
 }
 
+// From 48 rows on PARTS warps take a tile row: its left operand stays in registers for the row's tiles (i, i + t), t up to
+// half the tiles, columns wrapping around, which covers every pair once and gives each row as many. Calls f(place, c) for
+// each tile of A B.
+template <int NT, int PARTS, class F>
+__device__ __forceinline__ void strip(const double2 (&a)[NT], const double* B, int i, int part, F&& f) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll 1
+  for (int t = part; t <= NT / 2; t += PARTS) {
+    if (t == NT / 2 && i >= NT / 2) break;
+    const int j = i + t < NT ? i + t : i + t - NT;
+    const double* pb = B + j * NT * 64 + 2 * lane;
+    double c[2] = {0.0, 0.0}, c1[2] = {0.0, 0.0};
+#pragma unroll
+    for (int k = 0; k < NT; ++k) {
+      const double2 b = *reinterpret_cast<const double2*>(pb + 64 * k);
+      dmma(c, a[k].x, b.x);
+      dmma(c1, a[k].y, b.y);
+    }
+    c[0] += c1[0];
+    c[1] += c1[1];
+    f(Spot<NT>(i, j), c);
+  }
+}
+template <int NT>
+__device__ __forceinline__ void load_row(const double* A, int i, double2 (&a)[NT]) {
+#pragma unroll
+  for (int k = 0; k < NT; ++k)
+    a[k] = *reinterpret_cast<const double2*>(A + (i * NT + k) * 64 + 2 * (threadIdx.x & 31));
+}
+
 // Writes a tile and its mirror image.
 template <int NT>
-__device__ __forceinline__ void put_tile(double* M, int i, int j, const double (&c)[2]) {
-  const int lane = threadIdx.x & 31;
-  *reinterpret_cast<double2*>(M + (i * NT + j) * 64 + 2 * lane) = make_double2(c[0], c[1]);
-  if (i != j) {
-    double* m = M + (j * NT + i) * 64 + (lane & 3) * 16 + (lane >> 2);
-    m[0] = c[0];
-    m[8] = c[1];
+__device__ __forceinline__ void put_tile(double* M, const Spot<NT>& t, const double (&c)[2]) {
+  *reinterpret_cast<double2*>(M + t.own) = make_double2(c[0], c[1]);
+  if (!t.diagonal) {
+    M[t.mirror] = c[0];
+    M[t.mirror + 8] = c[1];
   }
 }
 
@@ -473,7 +526,7 @@ __device__ __forceinline__ void put_tile(double* M, int i, int j, const double (
 // product with x may then be fp32, whose d roundings stay near 2^-22 of the result. Gradients of low rank have entries
 // up to 485, and the sum cancels them.
 constexpr double kMaxPlain = 8.0;
-template <int NT>
+template <int NT, int WARPS>
 __device__ bool iterate(const Args& a, double* G, double* work, double*& P) {
   using D_ = Dims<NT>;
   double *S = work, *V = work + D_::MAT, *M = work + 2 * D_::MAT;
@@ -483,44 +536,85 @@ __device__ bool iterate(const Args& a, double* G, double* work, double*& P) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) tr += __shfl_xor_sync(0xffffffffu, tr, o);
   const double inv = 1.0 / (sqrt(tr) + a.eps);
+  // a warp's tiles: of S and of G' (R1 rounds), and of P' and V together (R2 rounds)
+  constexpr int R1 = (D_::TILES + WARPS - 1) / WARPS, R2 = (2 * D_::TILES + WARPS - 1) / WARPS;
   double sc = inv * inv;  // the first step's G still has to be scaled by it
   for (int step = 0; step < a.steps; ++step) {
     const double ca = a.coef[step][0], cb = a.coef[step][1] * sc, cc = a.coef[step][2] * sc * sc;
     const bool last = step + 1 == a.steps;
     double *from = M + ((step + 1) & 1) * D_::MAT, *to = M + (step & 1) * D_::MAT;
-    for (int n = warp; n < D_::TILES; n += kWarps) {
-      int i, j;
-      tile_of<NT>(n, i, j);
-      const double2 g = *reinterpret_cast<const double2*>(G + (i * NT + j) * 64 + 2 * lane);
-      double c[2];
-      product<NT>(G, G, i, j, c);
+    if constexpr (NT >= 6) {
       const int r = lane >> 2, k = 2 * (lane & 3);
-      c[0] = cb * g.x + cc * c[0] + (i == j && r == k ? ca : 0.0);
-      c[1] = cb * g.y + cc * c[1] + (i == j && r == k + 1 ? ca : 0.0);
-      put_tile<NT>(S, i, j, c);
-      if (step == 0) put_tile<NT>(to, i, j, c);
-    }
-    __syncthreads();
-    // P' = S P (from the second step on) and V = S G (but in the last), each tile by its own warp
-    const int np = step ? D_::TILES : 0, nv = last ? 0 : D_::TILES;
-    for (int n = warp; n < np + nv; n += kWarps) {
-      const bool isp = n < np;
-      int i, j;
-      tile_of<NT>(isp ? n : n - np, i, j);
-      double c[2];
-      product<NT>(S, isp ? from : G, i, j, c);
-      put_tile<NT>(isp ? to : V, i, j, c);
-    }
-    if (last) break;
-    __syncthreads();
-    for (int n = warp; n < D_::TILES; n += kWarps) {
-      int i, j;
-      tile_of<NT>(n, i, j);
-      double c[2];
-      product<NT>(S, V, i, j, c);
-      c[0] *= sc;
-      c[1] *= sc;
-      put_tile<NT>(G, i, j, c);
+      constexpr int PARTS = WARPS / NT;  // warps of a tile row
+      const int line = warp % NT, part = warp / NT;
+      double2 row[NT];
+      if (part < PARTS) {
+        load_row<NT>(G, line, row);
+        strip<NT, PARTS>(row, G, line, part, [&](const Spot<NT>& t, double (&c)[2]) {
+          const double2 g = *reinterpret_cast<const double2*>(G + t.own);
+          c[0] = cc * c[0] + (cb * g.x + (t.diagonal && r == k ? ca : 0.0));
+          c[1] = cc * c[1] + (cb * g.y + (t.diagonal && r == k + 1 ? ca : 0.0));
+          put_tile<NT>(S, t, c);
+          if (step == 0) put_tile<NT>(to, t, c);
+        });
+      }
+      __syncthreads();
+      if (part < PARTS) {
+        load_row<NT>(S, line, row);
+        if (!last) strip<NT, PARTS>(row, G, line, part, [&](const Spot<NT>& t, double (&c)[2]) { put_tile<NT>(V, t, c); });
+        if (step) strip<NT, PARTS>(row, from, line, part, [&](const Spot<NT>& t, double (&c)[2]) { put_tile<NT>(to, t, c); });
+      }
+      if (last) break;
+      __syncthreads();
+      if (part < PARTS)
+        strip<NT, PARTS>(row, V, line, part, [&](const Spot<NT>& t, double (&c)[2]) {
+          c[0] *= sc;
+          c[1] *= sc;
+          put_tile<NT>(G, t, c);
+        });
+    } else {
+#pragma unroll
+      for (int q = 0; q < R1; ++q) {
+        const int n = warp + q * WARPS;
+        if (n < D_::TILES) {
+          const Spot<NT> t(n);
+          const double2 g = *reinterpret_cast<const double2*>(G + t.own);
+          double c[2];
+          product<NT>(G, G, t, c);
+          const int r = lane >> 2, k = 2 * (lane & 3);
+          c[0] = cc * c[0] + (cb * g.x + (t.diagonal && r == k ? ca : 0.0));
+          c[1] = cc * c[1] + (cb * g.y + (t.diagonal && r == k + 1 ? ca : 0.0));
+          put_tile<NT>(S, t, c);
+          if (step == 0) put_tile<NT>(to, t, c);
+        }
+      }
+      __syncthreads();
+      // V = S G (but in the last step) and P' = S P (from the second on), each tile by its own warp
+#pragma unroll
+      for (int q = 0; q < R2; ++q) {
+        const int n = warp + q * WARPS;
+        const bool isv = n < D_::TILES;
+        if (isv ? !last : n < 2 * D_::TILES && step > 0) {
+          const Spot<NT> t(isv ? n : n - D_::TILES);
+          double c[2];
+          product<NT>(S, isv ? G : from, t, c);
+          put_tile<NT>(isv ? V : to, t, c);
+        }
+      }
+      if (last) break;
+      __syncthreads();
+#pragma unroll
+      for (int q = 0; q < R1; ++q) {
+        const int n = warp + q * WARPS;
+        if (n < D_::TILES) {
+          const Spot<NT> t(n);
+          double c[2];
+          product<NT>(S, V, t, c);
+          c[0] *= sc;
+          c[1] *= sc;
+          put_tile<NT>(G, t, c);
+        }
+      }
     }
     __syncthreads();
     sc = 1.0;
@@ -529,7 +623,7 @@ __device__ bool iterate(const Args& a, double* G, double* work, double*& P) {
   P = M + ((a.steps - 1) & 1) * D_::MAT;
   // the scale itself has to be a normal fp32 number with room for the sums
   bool plain = inv > 1e-30 && inv < 1e30;
-  for (int q = threadIdx.x; q < D_::MAT; q += kThreads) {
+  for (int q = threadIdx.x; q < D_::MAT; q += WARPS * 32) {
     plain = plain && fabs(P[q]) <= kMaxPlain;  // false for NaN
     P[q] *= inv;
   }
@@ -545,60 +639,91 @@ __device__ __forceinline__ void round_form(const double* P, float* Pf) {
   }
 }
 
-// x <- P x in place in fp64: a warp owns eight columns at a time.
+// x <- P x in place in fp64: a warp owns C groups of eight columns at a time. Up to 16 rows P stays in registers.
 template <int NT>
 __device__ __forceinline__ void apply(const double* P, float* x, int ld, int w) {
+  constexpr int C = NT <= 4 ? 2 : 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
   const double2* p = reinterpret_cast<const double2*>(P) + lane;
-  for (int j = warp * 8; j < w; j += kWarps * 8) {
-    double o[NT][2];
+  double2 held[NT <= 2 ? NT * NT : 1];
+  if (NT <= 2) {
 #pragma unroll
-    for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = 0.0;
+    for (int q = 0; q < NT * NT; ++q) held[q] = p[q * 32];
+  }
+  for (int j = warp * 8; j < w; j += kWarps * 8 * C) {
+    double o[C][NT][2];
+#pragma unroll
+    for (int g = 0; g < C; ++g)
+#pragma unroll
+      for (int i = 0; i < NT; ++i) o[g][i][0] = o[g][i][1] = 0.0;
     const float* b = x + 2 * c * ld + j + r;
 #pragma unroll
     for (int k = 0; k < NT; ++k) {
-      const double b0 = b[8 * k * ld], b1 = b[(8 * k + 1) * ld];
+      double v[C][2];
+#pragma unroll
+      for (int g = 0; g < C; ++g) {
+        const int at = j + g * kWarps * 8 < w ? g * kWarps * 8 : 0;  // a group past the end repeats the first
+        v[g][0] = b[8 * k * ld + at];
+        v[g][1] = b[(8 * k + 1) * ld + at];
+      }
       double2 f[NT];
 #pragma unroll
-      for (int i = 0; i < NT; ++i) f[i] = p[(i * NT + k) * 32];
+      for (int i = 0; i < NT; ++i) f[i] = NT <= 2 ? held[(i * NT + k) % (NT <= 2 ? NT * NT : 1)] : p[(i * NT + k) * 32];
 #pragma unroll
-      for (int i = 0; i < NT; ++i) dmma(o[i], f[i].x, b0);
+      for (int i = 0; i < NT; ++i)
 #pragma unroll
-      for (int i = 0; i < NT; ++i) dmma(o[i], f[i].y, b1);
+        for (int g = 0; g < C; ++g) dmma(o[g][i], f[i].x, v[g][0]);
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int g = 0; g < C; ++g) dmma(o[g][i], f[i].y, v[g][1]);
     }
     __syncwarp();
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
-      *reinterpret_cast<float2*>(x + (8 * i + r) * ld + j + 2 * c) = make_float2((float)o[i][0], (float)o[i][1]);
+    for (int g = 0; g < C; ++g)
+      if (j + g * kWarps * 8 < w) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+          *reinterpret_cast<float2*>(x + (8 * i + r) * ld + j + g * kWarps * 8 + 2 * c) =
+              make_float2((float)o[g][i][0], (float)o[g][i][1]);
+      }
   }
 }
 
-// The same in fp32: a thread owns two columns, and reads row k of P as a broadcast.
+// The same in fp32: a thread owns two columns and D / RG rows of the result, and reads row k of P as a broadcast. From 48
+// rows on (RG = 4) the four warps of a column write when all have read; w is at most kThreads * 2 / RG there.
 template <int NT>
 __device__ __forceinline__ void apply_plain(const float* Pf, float* x, int ld, int w) {
-  constexpr int D = NT * 8;
-  for (int j = threadIdx.x * 2; j < w; j += kThreads * 2) {
-    float o[D][2];
+  constexpr int D = NT * 8, RG = NT >= 6 ? 4 : 1, R = D / RG;
+  const int r0 = RG == 1 ? 0 : threadIdx.x / (kThreads / RG) * R;
+  for (int j = (threadIdx.x % (kThreads / RG)) * 2; j < w || RG > 1; j += kThreads * 2 / RG) {
+    float o[R][2];
 #pragma unroll
-    for (int i = 0; i < D; ++i) o[i][0] = o[i][1] = 0.f;
+    for (int i = 0; i < R; ++i) o[i][0] = o[i][1] = 0.f;
+    if (j < w) {
 #pragma unroll 4
-    for (int k = 0; k < D; ++k) {
-      const float2 v = *reinterpret_cast<const float2*>(x + k * ld + j);
+      for (int k = 0; k < D; ++k) {
+        const float2 v = *reinterpret_cast<const float2*>(x + k * ld + j);
 #pragma unroll
-      for (int i = 0; i < D; i += 4) {
-        const float4 p = *reinterpret_cast<const float4*>(Pf + k * D + i);
-        o[i][0] = fmaf(p.x, v.x, o[i][0]);
-        o[i][1] = fmaf(p.x, v.y, o[i][1]);
-        o[i + 1][0] = fmaf(p.y, v.x, o[i + 1][0]);
-        o[i + 1][1] = fmaf(p.y, v.y, o[i + 1][1]);
-        o[i + 2][0] = fmaf(p.z, v.x, o[i + 2][0]);
-        o[i + 2][1] = fmaf(p.z, v.y, o[i + 2][1]);
-        o[i + 3][0] = fmaf(p.w, v.x, o[i + 3][0]);
-        o[i + 3][1] = fmaf(p.w, v.y, o[i + 3][1]);
+        for (int i = 0; i < R; i += 4) {
+          const float4 p = *reinterpret_cast<const float4*>(Pf + k * D + r0 + i);
+          o[i][0] = fmaf(p.x, v.x, o[i][0]);
+          o[i][1] = fmaf(p.x, v.y, o[i][1]);
+          o[i + 1][0] = fmaf(p.y, v.x, o[i + 1][0]);
+          o[i + 1][1] = fmaf(p.y, v.y, o[i + 1][1]);
+          o[i + 2][0] = fmaf(p.z, v.x, o[i + 2][0]);
+          o[i + 2][1] = fmaf(p.z, v.y, o[i + 2][1]);
+          o[i + 3][0] = fmaf(p.w, v.x, o[i + 3][0]);
+          o[i + 3][1] = fmaf(p.w, v.y, o[i + 3][1]);
+        }
       }
     }
+    if (RG > 1) __syncthreads();
+    if (j < w) {
 #pragma unroll
-    for (int i = 0; i < D; ++i) *reinterpret_cast<float2*>(x + i * ld + j) = make_float2(o[i][0], o[i][1]);
+      for (int i = 0; i < R; ++i) *reinterpret_cast<float2*>(x + (r0 + i) * ld + j) = make_float2(o[i][0], o[i][1]);
+    }
+    if (RG > 1) break;
   }
 }
 
@@ -652,7 +777,7 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 ? 4 : 2) ortho_kernel(const 
   }
   __syncthreads();
   double* P;
-  if (iterate<NT>(a, G, work, P)) {
+  if (iterate<NT, kWarps>(a, G, work, P)) {
     float* Pf = reinterpret_cast<float*>(G);
     round_form<NT>(P, Pf);
     __syncthreads();
@@ -667,7 +792,7 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 ? 4 : 2) ortho_kernel(const 
 
 // Split: block b of a matrix takes the chunks b, b + blocks, ... of `cap` columns.
 template <int NT, typename T, bool MUON>
-__global__ void __launch_bounds__(kThreads, 2) gram_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(kThreads, NT == 6 ? 2 : 3) gram_kernel(const __grid_constant__ Args a) {
   using D_ = Dims<NT>;
   extern __shared__ __align__(16) double sm[];
   double* work = sm;
@@ -688,14 +813,20 @@ __global__ void __launch_bounds__(kThreads, 2) gram_kernel(const __grid_constant
   reduce_warps<NT>(acc, work, a.gram + (long long)blockIdx.x * D_::PART);
 }
 
+template <int NT>
+constexpr int form_warps() {
+  return NT >= 6 ? 16 : kWarps;
+}
+
 // One block per matrix: the parts in order, then P.
 template <int NT>
-__global__ void __launch_bounds__(kThreads) form_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(form_warps<NT>() * 32) form_kernel(const __grid_constant__ Args a) {
   using D_ = Dims<NT>;
+  constexpr int FT = form_warps<NT>() * 32;
   extern __shared__ __align__(16) double sm[];
   double *G = sm, *work = G + D_::MAT;
   const double* part = a.gram + (long long)blockIdx.x * a.blocks * D_::PART;
-  for (int q = threadIdx.x; q < D_::PART; q += kThreads) {
+  for (int q = threadIdx.x; q < D_::PART; q += FT) {
     double s = 0.0;
 #pragma unroll 8
     for (int b = 0; b < a.blocks; ++b) s += part[(long long)b * D_::PART + q];
@@ -703,14 +834,14 @@ __global__ void __launch_bounds__(kThreads) form_kernel(const __grid_constant__ 
   }
   __syncthreads();
   double* P;
-  const bool plain = iterate<NT>(a, G, work, P);
+  const bool plain = iterate<NT, form_warps<NT>()>(a, G, work, P);
   double* out = a.form + (long long)blockIdx.x * (D_::MAT + 2);
-  for (int q = threadIdx.x; q < D_::MAT; q += kThreads) out[q] = P[q];
+  for (int q = threadIdx.x; q < D_::MAT; q += FT) out[q] = P[q];
   if (threadIdx.x == 0) out[D_::MAT] = plain ? 1.0 : 0.0;
 }
 
 template <int NT, typename T, bool MUON>
-__global__ void __launch_bounds__(kThreads) product_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(kThreads, 3) product_kernel(const __grid_constant__ Args a) {
   using D_ = Dims<NT>;
   extern __shared__ __align__(16) double sm[];
   float* x = reinterpret_cast<float*>(sm + D_::MAT);
@@ -742,12 +873,12 @@ void set_cap(Args& a, int cap) {
 }
 
 template <typename F>
-int launch(F* kern, const Args& a, long long blocks, long long smem, int cluster, cudaStream_t st) {
+int launch(F* kern, const Args& a, long long blocks, int threads, long long smem, int cluster, cudaStream_t st) {
   SMELB_CHECK_ARG(blocks < (1LL << 31), kErrShape, "orthogonalize: %lld blocks", blocks);
   SMELB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)blocks);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = st;
   cudaLaunchAttribute at[1];
@@ -767,13 +898,14 @@ constexpr int kBlockCols = 512, kMaxBlocks = 8;
 // Whether matrices of this size are held by a cluster: up to 32 rows, and no more columns than eight blocks hold.
 bool resident(int nt, int L) { return nt <= 4 && L <= kBlockCols * kMaxBlocks; }
 
-constexpr int kSplitCap = 128;
+static_assert(kSplitCap <= kThreads * 2 / 4, "apply_plain takes a chunk at once from 48 rows on");
 
-// Blocks for one matrix of the split way.
+// Blocks for one matrix of the split way: as many chunks to each as leave eight blocks for an SM, and at most two blocks on
+// every SM for one matrix (their partial Gram matrices are added by one block).
 int split_blocks(long long matrices, int L) {
   const long long chunks = (L + kSplitCap - 1) / kSplitCap;
-  const long long want = (148 * 4 + matrices - 1) / matrices;  // four blocks to an SM
-  return (int)std::max<long long>(1, std::min<long long>(chunks, std::min<long long>(want, 296)));
+  const long long per = std::max({1LL, chunks * matrices / (148 * 8), (chunks + 295) / 296});
+  return (int)((chunks + per - 1) / per);
 }
 
 template <int NT, typename T, bool MUON>
@@ -784,7 +916,7 @@ int run_resident(Args& a, long long matrices, int maxL, cudaStream_t st) {
   a.blocks = c;
   set_cap(a, ((maxL + c - 1) / c + 31) / 32 * 32);
   const long long smem = (long long)(D_::MAT + D_::PART + D_::WORK) * 8 + (long long)NT * 8 * pitch(a.cap) * 4;
-  return launch(ortho_kernel<NT, T, MUON>, a, matrices * c, smem, c, st);
+  return launch(ortho_kernel<NT, T, MUON>, a, matrices * c, kThreads, smem, c, st);
 }
 
 template <int NT, typename T, bool MUON>
@@ -795,9 +927,9 @@ int run_split(Args& a, long long matrices, int maxL, double* ws, cudaStream_t st
   a.gram = ws;
   a.form = ws + matrices * a.blocks * D_::PART;
   const long long x = (long long)NT * 8 * pitch(a.cap) * 4;
-  int rc = launch(gram_kernel<NT, T, MUON>, a, matrices * a.blocks, (long long)D_::BUFS * D_::PART * 8 + x, 1, st);
-  if (rc == kOk) rc = launch(form_kernel<NT>, a, matrices, (long long)(D_::MAT + D_::WORK) * 8, 1, st);
-  if (rc == kOk) rc = launch(product_kernel<NT, T, MUON>, a, matrices * a.blocks, (long long)D_::MAT * 8 + x, 1, st);
+  int rc = launch(gram_kernel<NT, T, MUON>, a, matrices * a.blocks, kThreads, (long long)D_::BUFS * D_::PART * 8 + x, 1, st);
+  if (rc == kOk) rc = launch(form_kernel<NT>, a, matrices, form_warps<NT>() * 32, (long long)(D_::MAT + D_::WORK) * 8, 1, st);
+  if (rc == kOk) rc = launch(product_kernel<NT, T, MUON>, a, matrices * a.blocks, kThreads, (long long)D_::MAT * 8 + x, 1, st);
   return rc;
 }
 
