@@ -25,6 +25,7 @@ namespace {
 
 constexpr int kThreads = 256, kWarps = 8;
 constexpr int kSplitCap = 128;  // columns of a chunk of the split way
+constexpr int kDevErrWaitCluster = 16;  // a block waiting for its cluster's parts of the Gram matrix
 constexpr int kMaxSteps = 16, kMaxTensors = 48, kMaxD = 64;
 
 struct Tensor {
@@ -47,6 +48,7 @@ struct Args {
   float mu, omu, decay;  // omu: 1 - momentum, from 64 bits
   int nesterov;
   double eps;
+  int* err;      // status words
   double* gram;  // split: [matrix][block][PART] partial Gram matrices
   double* form;  // split: [matrix][NT * NT * 64 + 1] P and whether it is plain
   double coef[kMaxSteps][3];
@@ -64,10 +66,15 @@ struct Dims {
   static constexpr int GROUPS = NT == 8 ? 4 : 1;        // tile groups among the warps (accumulators in registers)
   static constexpr int ACC = GROUPS == 1 ? TILES : NT + 1;  // tiles of a group
   static constexpr int KG = kWarps / GROUPS;            // warps that split the columns
-  static constexpr int BUFS = KG < 4 ? KG : 4;          // partial Gram matrices in shared memory at once
+  static constexpr int BUFS = NT >= 3 ? 2 : 4;          // the warps' partial Gram matrices in shared memory at once
   static constexpr int MAT = NT * NT * 64;              // doubles of one matrix
   static constexpr int PART = TILES * 64;               // doubles of one packed upper triangle
-  static constexpr int WORK = 4 * MAT > BUFS * PART ? 4 * MAT : BUFS * PART;  // S, V and two P; partial sums before
+  static constexpr int POLY = 4 * MAT;                  // S, V and two P
+  // doubles of the work space that S, V and P share with what comes before them: the warps' partial sums, then one
+  // from each block of the cluster
+  static constexpr int work(int cluster) {
+    return POLY > (BUFS + cluster) * PART ? POLY : (BUFS + cluster) * PART;
+  }
 };
 
 // Pitch of the columns in shared memory: 4 mod 32, so the operands of the Gram product (8 rows x 4 columns) and of the
@@ -81,13 +88,16 @@ __device__ __forceinline__ void dmma(double (&c)[2], double a, double b) {
 }
 
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
-__device__ __forceinline__ double ld_cluster(const double* p, int rank) {
-  uint32_t a;
-  double v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
-  asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(a));
-  return v;
+// 16 bytes into the same place of the cluster's block `rank`, counted by its barrier `bar`.
+__device__ __forceinline__ void push(double* to, uint64_t* bar, int rank, double a, double b) {
+  uint32_t at, mb;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(to)), "r"(rank));
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(mb) : "r"(smem_u32(bar)), "r"(rank));
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.f64 [%0], {%1, %2}, [%3];" ::"r"(at), "d"(a),
+               "d"(b), "r"(mb)
+               : "memory");
 }
 
 __device__ __forceinline__ float to_f(float v) { return v; }
@@ -137,24 +147,24 @@ __device__ __forceinline__ uint4 repack(const Vec<bf16>& o) {
 
 // The vectors of N elements of a block's columns [j0, j0 + w): vector q of a wide matrix is row q / (cap / N), columns from
 // N (q % (cap / N)); a tall matrix is contiguous, element e of it is (i, j) = (e % d, e / d).
-template <int N>
+template <int N, bool TALL>
 struct Place {
   int i, j;
-  long long at;  // offset in memory from column j0
   bool live;
   __device__ __forceinline__ Place(const Args& a, const Tensor& t, int w, int q) {
-    if (t.tall) {
-      const int e = q * N;
-      j = (int)__umulhi((uint32_t)e, t.by_d);
-      i = e - j * t.d;
-      at = e;
+    if (TALL) {
+      j = (int)__umulhi((uint32_t)(q * N), t.by_d);
+      i = q * N - j * t.d;
       live = j < w;
     } else {
       i = (int)__umulhi((uint32_t)q, a.by_v[N == 8]);
       j = (q - i * (a.cap / N)) * N;
-      at = (long long)i * t.L + j;
       live = i < t.d && j < w;
     }
+  }
+  // offset in memory from column j0
+  __device__ __forceinline__ long long at(const Tensor& t) const {
+    return TALL ? (long long)(j * t.d + i) : (long long)i * t.L + j;
   }
 };
 template <int N>
@@ -163,18 +173,27 @@ __device__ __forceinline__ int places(const Args& a, const Tensor& t, int w) {
 }
 
 // The N elements of a vector: v -> x (PUT) or x -> v.
-template <bool PUT, int N>
-__device__ __forceinline__ void move(const Tensor& t, const Place<N>& at, float* x, int ld, float (&v)[N]) {
-  if (t.tall) {
+template <bool PUT, int N, bool TALL>
+__device__ __forceinline__ void move(const Tensor& t, const Place<N, TALL>& at, float* x, int ld, float (&v)[N]) {
+  if (TALL) {
+    float* c = x + at.i * ld + at.j;
+    if (t.d % N == 0) {
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        if (PUT) c[k * ld] = v[k];
+        else v[k] = c[k * ld];
+      }
+      return;
+    }
     int i = at.i;
-    float* c = x + at.j;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-      if (PUT) c[i * ld] = v[k];
-      else v[k] = c[i * ld];
+      if (PUT) *c = v[k];
+      else v[k] = *c;
+      c += ld;
       if (++i == t.d) {
         i = 0;
-        ++c;
+        c += 1 - t.d * ld;
       }
     }
   } else {
@@ -203,50 +222,59 @@ __device__ __forceinline__ bool vectors(const Tensor& t, long long base, int w) 
   return (at & 15) == 0 && (t.tall ? (w * t.d) % N == 0 : t.L % N == 0 && w % N == 0);
 }
 
+template <typename T, bool MUON, bool TALL>
+__device__ __forceinline__ void load_vectors(const Args& a, const Tensor& t, const T* g, float* m, int w, float* x,
+                                             int ld, bool first) {
+  constexpr int N = Vec<T>::N, U = MUON && N == 8 ? 2 : 4;  // vectors in flight per thread
+  const int end = places<N>(a, t, w);
+  for (int q0 = threadIdx.x; q0 < end; q0 += kThreads * U) {
+    uint4 rg[U], rm[U][N / 4];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const Place<N, TALL> at(a, t, w, q0 + u * kThreads);
+      if (at.live) {
+        rg[u] = __ldg(reinterpret_cast<const uint4*>(g + at.at(t)));
+        if (MUON) {
+#pragma unroll
+          for (int k = 0; k < N / 4; ++k) rm[u][k] = *reinterpret_cast<const uint4*>(m + at.at(t) + 4 * k);
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const Place<N, TALL> at(a, t, w, q0 + u * kThreads);
+      if (at.live) {
+        Vec<T> v;
+        unpack(rg[u], v);
+        if (MUON) {
+#pragma unroll
+          for (int k = 0; k < N / 4; ++k) {
+            Vec<float> b;
+            unpack(rm[u][k], b);
+#pragma unroll
+            for (int l = 0; l < 4; ++l) v.v[4 * k + l] = update(a, v.v[4 * k + l], b.v[l], first);
+            if (first) *reinterpret_cast<uint4*>(m + at.at(t) + 4 * k) = repack(b);
+          }
+        }
+        move<true>(t, at, x, ld, v.v);
+      }
+    }
+  }
+}
+
 // Columns [j0, j0 + w) (j0 a multiple of 8) into x, zeros up to the next multiple of 8 and in the rows that fill the
 // tiles. `first`: the momentum buffer is still the old one.
 template <int NT, typename T, bool MUON>
 __device__ __forceinline__ void load_slice(const Args& a, const Tensor& t, long long base, int j0, int w, float* x,
                                            int ld, bool first) {
-  constexpr int N = Vec<T>::N, U = MUON && N == 8 ? 2 : 4;  // vectors in flight per thread
+  const bool vec = vectors<T, MUON>(t, base, w);
   base += t.tall ? (long long)j0 * t.d : j0;
   const T* g = reinterpret_cast<const T*>(t.g) + base;
   float* m = MUON ? t.m + base : nullptr;
-  if (vectors<T, MUON>(t, base, w)) {
-    const int end = places<N>(a, t, w);
-    for (int q0 = threadIdx.x; q0 < end; q0 += kThreads * U) {
-      uint4 rg[U], rm[U][N / 4];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const Place<N> at(a, t, w, q0 + u * kThreads);
-        if (at.live) {
-          rg[u] = __ldg(reinterpret_cast<const uint4*>(g + at.at));
-          if (MUON) {
-#pragma unroll
-            for (int k = 0; k < N / 4; ++k) rm[u][k] = *reinterpret_cast<const uint4*>(m + at.at + 4 * k);
-          }
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const Place<N> at(a, t, w, q0 + u * kThreads);
-        if (at.live) {
-          Vec<T> v;
-          unpack(rg[u], v);
-          if (MUON) {
-#pragma unroll
-            for (int k = 0; k < N / 4; ++k) {
-              Vec<float> b;
-              unpack(rm[u][k], b);
-#pragma unroll
-              for (int l = 0; l < 4; ++l) v.v[4 * k + l] = update(a, v.v[4 * k + l], b.v[l], first);
-              if (first) *reinterpret_cast<uint4*>(m + at.at + 4 * k) = repack(b);
-            }
-          }
-          move<true>(t, at, x, ld, v.v);
-        }
-      }
-    }
+  if (vec && t.tall) {
+    load_vectors<T, MUON, true>(a, t, g, m, w, x, ld, first);
+  } else if (vec) {
+    load_vectors<T, MUON, false>(a, t, g, m, w, x, ld, first);
   } else {
     for (int q = threadIdx.x; q < w * t.d; q += kThreads) {
       const int i = t.tall ? q % t.d : q / w, j = t.tall ? q / t.d : q % w;
@@ -277,36 +305,44 @@ __device__ __forceinline__ float result(const Args& a, const Tensor& t, float o,
   return MUON ? fmaf(-t.step, o, p * a.decay) : o;
 }
 
+template <typename T, bool MUON, bool TALL>
+__device__ __forceinline__ void store_vectors(const Args& a, const Tensor& t, T* p, int w, float* x, int ld) {
+  constexpr int N = Vec<T>::N, U = 4;
+  const int end = places<N>(a, t, w);
+  for (int q0 = threadIdx.x; q0 < end; q0 += kThreads * U) {
+    uint4 rp[U];
+    if (MUON) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const Place<N, TALL> at(a, t, w, q0 + u * kThreads);
+        if (at.live) rp[u] = *reinterpret_cast<const uint4*>(p + at.at(t));
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const Place<N, TALL> at(a, t, w, q0 + u * kThreads);
+      if (at.live) {
+        Vec<T> v, was{};
+        if (MUON) unpack(rp[u], was);
+        move<false>(t, at, x, ld, v.v);
+#pragma unroll
+        for (int k = 0; k < N; ++k) v.v[k] = result<MUON>(a, t, v.v[k], was.v[k]);
+        *reinterpret_cast<uint4*>(p + at.at(t)) = repack(v);
+      }
+    }
+  }
+}
+
 template <typename T, bool MUON>
 __device__ __forceinline__ void store_slice(const Args& a, const Tensor& t, long long base, int j0, int w, float* x,
                                             int ld) {
-  constexpr int N = Vec<T>::N, U = 4;
+  const bool vec = vectors<T, MUON>(t, base, w);
   base += t.tall ? (long long)j0 * t.d : j0;
   T* p = reinterpret_cast<T*>(t.p) + base;
-  if (vectors<T, MUON>(t, base, w)) {
-    const int end = places<N>(a, t, w);
-    for (int q0 = threadIdx.x; q0 < end; q0 += kThreads * U) {
-      uint4 rp[U];
-      if (MUON) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const Place<N> at(a, t, w, q0 + u * kThreads);
-          if (at.live) rp[u] = *reinterpret_cast<const uint4*>(p + at.at);
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const Place<N> at(a, t, w, q0 + u * kThreads);
-        if (at.live) {
-          Vec<T> v, was{};
-          if (MUON) unpack(rp[u], was);
-          move<false>(t, at, x, ld, v.v);
-#pragma unroll
-          for (int k = 0; k < N; ++k) v.v[k] = result<MUON>(a, t, v.v[k], was.v[k]);
-          *reinterpret_cast<uint4*>(p + at.at) = repack(v);
-        }
-      }
-    }
+  if (vec && t.tall) {
+    store_vectors<T, MUON, true>(a, t, p, w, x, ld);
+  } else if (vec) {
+    store_vectors<T, MUON, false>(a, t, p, w, x, ld);
   } else {
     for (int q = threadIdx.x; q < w * t.d; q += kThreads) {
       const int i = t.tall ? q % t.d : q / w, j = t.tall ? q / t.d : q % w;
@@ -398,25 +434,35 @@ __device__ __forceinline__ void pack_group(int grp, double* part, double (&acc)[
   }
 }
 
-// The warps' partial Gram matrices into `part`: halved until BUFS are left, then added in order. `work`: BUFS parts.
-template <int NT>
-__device__ __forceinline__ void reduce_warps(double (&acc)[Dims<NT>::ACC][2], double* work, double* part) {
+// The warps' partial Gram matrices: halved until BUFS are left, then added in order. Calls f(q, sum q, sum q + 1) for the
+// even q of the packed upper triangle. `work`: BUFS parts.
+template <int NT, class F>
+__device__ __forceinline__ void reduce_warps(double (&acc)[Dims<NT>::ACC][2], double* work, F&& f) {
   using D_ = Dims<NT>;
   const int warp = threadIdx.x >> 5, grp = warp % D_::GROUPS, kg = warp / D_::GROUPS;
 #pragma unroll
   for (int h = D_::KG; h > D_::BUFS; h /= 2) {
-    if (kg >= h / 2 && kg < h) pack_group<NT, false>(grp, work + (kg - h / 2) * D_::PART, acc);
-    __syncthreads();
-    if (kg < h / 2) pack_group<NT, true>(grp, work + kg * D_::PART, acc);
-    __syncthreads();
+    // the upper half goes through the buffers, as many at a time as there are
+#pragma unroll
+    for (int o = h / 2; o < h; o += D_::BUFS) {
+      if (kg >= o && kg < o + D_::BUFS) pack_group<NT, false>(grp, work + (kg - o) * D_::PART, acc);
+      __syncthreads();
+      const int to = o - h / 2;
+      if (kg >= to && kg < to + D_::BUFS && kg < h / 2) pack_group<NT, true>(grp, work + (kg - to) * D_::PART, acc);
+      __syncthreads();
+    }
   }
   if (kg < D_::BUFS) pack_group<NT, false>(grp, work + kg * D_::PART, acc);
   __syncthreads();
-  for (int q = threadIdx.x; q < D_::PART; q += kThreads) {
-    double s = work[q];
+  for (int q = threadIdx.x * 2; q < D_::PART; q += kThreads * 2) {
+    double2 s = *reinterpret_cast<const double2*>(work + q);
 #pragma unroll
-    for (int b = 1; b < D_::BUFS; ++b) s += work[b * D_::PART + q];
-    part[q] = s;
+    for (int b = 1; b < D_::BUFS; ++b) {
+      const double2 v = *reinterpret_cast<const double2*>(work + b * D_::PART + q);
+      s.x += v.x;
+      s.y += v.y;
+    }
+    f(q, s.x, s.y);
   }
 }
 
@@ -739,14 +785,25 @@ __device__ __forceinline__ const Tensor& tensor_of(const Args& a, long long mat,
   return a.t[ti];
 }
 
-// Resident: the blocks of a cluster hold one matrix, `cap` columns each at most.
+// Resident: the blocks of a cluster hold one matrix, `cap` columns each at most. Their parts of the Gram matrix go to every
+// block's shared memory by asynchronous stores that the receiver's barrier counts: one way, and without the fence over
+// the stores to the momentum buffer that a cluster barrier would need.
 template <int NT, typename T, bool MUON>
 __global__ void __launch_bounds__(kThreads, NT <= 2 ? 4 : 2) ortho_kernel(const __grid_constant__ Args a) {
   using D_ = Dims<NT>;
   extern __shared__ __align__(16) double sm[];
-  double *G = sm, *part = G + D_::MAT, *work = part + D_::PART;
-  float* x = reinterpret_cast<float*>(work + D_::WORK);
+  __shared__ __align__(8) uint64_t bar;
+  double *G = sm, *work = G + D_::MAT, *slots = work + D_::BUFS * D_::PART;
+  float* x = reinterpret_cast<float*>(work + D_::work(a.blocks));
   const int rank = blockIdx.x % a.blocks, ld = pitch(a.cap);
+  if (a.blocks > 1) {
+    if (threadIdx.x == 0) {
+      mbar_init(&bar, 1);
+      fence_mbar_init();
+      mbar_arrive_expect_tx(&bar, (uint32_t)(a.blocks * D_::PART * sizeof(double)));
+    }
+    cluster_arrive();
+  }
   long long base;
   const Tensor& t = tensor_of(a, blockIdx.x / a.blocks, base);
   const int slice = ((t.L + a.blocks - 1) / a.blocks + 7) & ~7;
@@ -758,22 +815,24 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 ? 4 : 2) ortho_kernel(const 
   if (w) load_slice<NT, T, MUON>(a, t, base, j0, w, x, ld, true);
   __syncthreads();
   gram<NT, 0>(x, ld, w, threadIdx.x >> 5, acc);
-  reduce_warps<NT>(acc, work, part);
   if (a.blocks > 1) {
-    cluster_arrive();
-    cluster_wait();
+    cluster_wait();  // every block's barrier is set up
+    reduce_warps<NT>(acc, work, [&](int q, double v0, double v1) {
+      for (int r = 0; r < a.blocks; ++r) push(slots + rank * D_::PART + q, &bar, r, v0, v1);
+    });
+    mbar_wait(&bar, 0, a.err, kDevErrWaitCluster, blockIdx.x);
     for (int q = threadIdx.x; q < D_::PART; q += kThreads) {
-      double v[8], s = 0.0;
-#pragma unroll
-      for (int r = 0; r < 8; ++r) v[r] = r < a.blocks ? ld_cluster(part + q, r) : 0.0;
-#pragma unroll
-      for (int r = 0; r < 8; ++r) s += v[r];
+      double s = 0.0;
+#pragma unroll 4
+      for (int r = 0; r < a.blocks; ++r) s += slots[r * D_::PART + q];
       spread<NT>(G, q, s);
     }
-    cluster_arrive();  // this block has read the others' parts
+    cluster_arrive_relaxed();  // for the exit: this block's pushes are under way
   } else {
-    __syncthreads();
-    for (int q = threadIdx.x; q < D_::PART; q += kThreads) spread<NT>(G, q, part[q]);
+    reduce_warps<NT>(acc, work, [&](int q, double v0, double v1) {
+      spread<NT>(G, q, v0);
+      spread<NT>(G, q + 1, v1);
+    });
   }
   __syncthreads();
   double* P;
@@ -787,12 +846,12 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 ? 4 : 2) ortho_kernel(const 
   }
   __syncthreads();
   if (w) store_slice<T, MUON>(a, t, base, j0, w, x, ld);
-  if (a.blocks > 1) cluster_wait();  // its part stays until every block has read it
+  if (a.blocks > 1) cluster_wait();
 }
 
 // Split: block b of a matrix takes the chunks b, b + blocks, ... of `cap` columns.
 template <int NT, typename T, bool MUON>
-__global__ void __launch_bounds__(kThreads, NT == 6 ? 2 : 3) gram_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(kThreads, NT == 6 || MUON || sizeof(T) == 2 ? 2 : 3) gram_kernel(const __grid_constant__ Args a) {
   using D_ = Dims<NT>;
   extern __shared__ __align__(16) double sm[];
   double* work = sm;
@@ -810,7 +869,10 @@ __global__ void __launch_bounds__(kThreads, NT == 6 ? 2 : 3) gram_kernel(const _
     gram_group<NT>(warp % D_::GROUPS, x, ld, w, warp / D_::GROUPS, acc);
     __syncthreads();
   }
-  reduce_warps<NT>(acc, work, a.gram + (long long)blockIdx.x * D_::PART);
+  double* part = a.gram + (long long)blockIdx.x * D_::PART;
+  reduce_warps<NT>(acc, work, [&](int q, double v0, double v1) {
+    *reinterpret_cast<double2*>(part + q) = make_double2(v0, v1);
+  });
 }
 
 template <int NT>
@@ -841,7 +903,7 @@ __global__ void __launch_bounds__(form_warps<NT>() * 32) form_kernel(const __gri
 }
 
 template <int NT, typename T, bool MUON>
-__global__ void __launch_bounds__(kThreads, 3) product_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(kThreads, NT >= 6 && !MUON && sizeof(T) == 4 ? 3 : 2) product_kernel(const __grid_constant__ Args a) {
   using D_ = Dims<NT>;
   extern __shared__ __align__(16) double sm[];
   float* x = reinterpret_cast<float*>(sm + D_::MAT);
@@ -891,12 +953,20 @@ int launch(F* kern, const Args& a, long long blocks, int threads, long long smem
   return kOk;
 }
 
-// Columns of a resident block at most: 45 KB for 16 rows (four blocks to an SM; 1024 columns in two ran 7% slower on 1548
-// matrices of 16 x 512 .. 2048), 112 KB for 32 (two blocks).
-constexpr int kBlockCols = 512, kMaxBlocks = 8;
+// Columns of a resident block at most: 47 KB for 16 rows (four blocks to an SM; 1024 columns in two ran 7% slower on 1548
+// matrices of 16 x 512 .. 2048), 104 KB for 32 (two blocks).
+constexpr int kMaxBlocks = 8;
+constexpr int block_cols(int nt) { return nt <= 2 ? 512 : 352; }
 
 // Whether matrices of this size are held by a cluster: up to 32 rows, and no more columns than eight blocks hold.
-bool resident(int nt, int L) { return nt <= 4 && L <= kBlockCols * kMaxBlocks; }
+bool resident(int nt, int L) { return nt <= 4 && L <= block_cols(nt) * kMaxBlocks; }
+
+// Blocks that a resident matrix needs.
+int blocks_needed(int nt, int L) {
+  int c = 1;
+  while (L > block_cols(nt) * c) c *= 2;
+  return c;
+}
 
 static_assert(kSplitCap <= kThreads * 2 / 4, "apply_plain takes a chunk at once from 48 rows on");
 
@@ -911,11 +981,12 @@ int split_blocks(long long matrices, int L) {
 template <int NT, typename T, bool MUON>
 int run_resident(Args& a, long long matrices, int maxL, cudaStream_t st) {
   using D_ = Dims<NT>;
-  int c = 1;
-  while (c < kMaxBlocks && (maxL > kBlockCols * c || (maxL > 256 * c && matrices * c < 296))) c *= 2;
+  // few matrices: more blocks for each, down to 256 columns, until two are on every SM
+  int c = blocks_needed(NT, maxL);
+  while (c < kMaxBlocks && maxL > 256 * c && matrices * c < 296) c *= 2;
   a.blocks = c;
   set_cap(a, ((maxL + c - 1) / c + 31) / 32 * 32);
-  const long long smem = (long long)(D_::MAT + D_::PART + D_::WORK) * 8 + (long long)NT * 8 * pitch(a.cap) * 4;
+  const long long smem = (long long)(D_::MAT + D_::work(c)) * 8 + (long long)NT * 8 * pitch(a.cap) * 4;
   return launch(ortho_kernel<NT, T, MUON>, a, matrices * c, kThreads, smem, c, st);
 }
 
@@ -928,7 +999,7 @@ int run_split(Args& a, long long matrices, int maxL, double* ws, cudaStream_t st
   a.form = ws + matrices * a.blocks * D_::PART;
   const long long x = (long long)NT * 8 * pitch(a.cap) * 4;
   int rc = launch(gram_kernel<NT, T, MUON>, a, matrices * a.blocks, kThreads, (long long)D_::BUFS * D_::PART * 8 + x, 1, st);
-  if (rc == kOk) rc = launch(form_kernel<NT>, a, matrices, form_warps<NT>() * 32, (long long)(D_::MAT + D_::WORK) * 8, 1, st);
+  if (rc == kOk) rc = launch(form_kernel<NT>, a, matrices, form_warps<NT>() * 32, (long long)(D_::MAT + D_::POLY) * 8, 1, st);
   if (rc == kOk) rc = launch(product_kernel<NT, T, MUON>, a, matrices * a.blocks, kThreads, (long long)D_::MAT * 8 + x, 1, st);
   return rc;
 }
@@ -967,30 +1038,47 @@ int check_shapes(const smelb_muon_tensor* t, int64_t n, const char* what) {
   return kOk;
 }
 
-// Calls f(row tiles, held, first tensor.., matrices, longest side) for every launch: tensors of the same row tiles and the
-// same way, at most kMaxTensors. The list of a launch is idx[0 .. count).
+// Calls f(row tiles, held, the launch's tensors idx[0 .. count), matrices, longest side) for every launch: tensors of the
+// same row tiles and way, at most kMaxTensors. Resident matrices that fill the SMs more than once go by the blocks that
+// they need (a short matrix spread over the blocks of a long one forms P in each of them); fewer take one launch.
 template <typename F>
 int for_launches(const smelb_muon_tensor* t, int64_t n, F&& f) {
-  for (int nt : kTileCounts)
-    for (int held = 0; held < 2; ++held) {
+  for (int nt : kTileCounts) {
+    long long held = 0;
+    bool any = false;
+    int most = 1;
+    for (int64_t i = 0; i < n; ++i) {
+      const int d = (int)std::min(t[i].rows, t[i].cols), L = (int)std::max(t[i].rows, t[i].cols);
+      if (t[i].batch == 0 || tiles_for(d) != nt) continue;
+      any = true;
+      if (resident(nt, L)) {
+        held += t[i].batch;
+        most = std::max(most, blocks_needed(nt, L));
+      }
+    }
+    if (!any) continue;
+    const bool apart = held * most > 148 * 4;
+    for (int way = 0; way <= kMaxBlocks; way = way ? 2 * way : 1) {  // 0: split; else blocks of a resident matrix
       int64_t idx[kMaxTensors];
       int count = 0, maxL = 0;
       long long matrices = 0;
       for (int64_t i = 0; i < n; ++i) {
         const int d = (int)std::min(t[i].rows, t[i].cols), L = (int)std::max(t[i].rows, t[i].cols);
-        if (t[i].batch == 0 || tiles_for(d) != nt || resident(nt, L) != (held != 0)) continue;
+        if (t[i].batch == 0 || tiles_for(d) != nt) continue;
+        if (way != (!resident(nt, L) ? 0 : apart ? blocks_needed(nt, L) : 1)) continue;
         idx[count++] = i;
         matrices += t[i].batch;
         maxL = std::max(maxL, L);
         if (count == kMaxTensors) {
-          if (int rc = f(nt, held != 0, idx, count, matrices, maxL)) return rc;
+          if (int rc = f(nt, way != 0, idx, count, matrices, maxL)) return rc;
           count = maxL = 0;
           matrices = 0;
         }
       }
       if (count)
-        if (int rc = f(nt, held != 0, idx, count, matrices, maxL)) return rc;
+        if (int rc = f(nt, way != 0, idx, count, matrices, maxL)) return rc;
     }
+  }
   return kOk;
 }
 
@@ -1020,7 +1108,13 @@ int run(const smelb_muon_tensor* t, int64_t n, int dtype, bool muon, double lr, 
   SMELB_CHECK_ARG(ws_bytes >= need && (ws || !need), kErrWorkspace, "%s: workspace %lld bytes, %lld needed", what,
                   (long long)ws_bytes, need);
   SMELB_CHECK_ARG(((uintptr_t)ws & 255) == 0, kErrArg, "%s: workspace must be 256-byte aligned", what);
+  bool any = false;
+  for (int64_t i = 0; i < n; ++i) any = any || t[i].batch > 0;
+  if (!any) return kOk;
+  int dev = 0;
+  SMELB_CUDA(cudaGetDevice(&dev));
   Args a{};
+  a.err = device_status_on(dev, st);
   a.steps = steps;
   a.mu = (float)mu;
   a.omu = (float)(1.0 - mu);
