@@ -42,7 +42,8 @@ struct Tensor {
 struct Args {
   Tensor t[kMaxTensors];
   int n, steps;
-  int blocks;        // blocks of one matrix
+  int blocks;        // blocks of one matrix; resident: a power of two, 2^shift
+  int shift;
   int cap;           // columns that a block holds at once (a multiple of 32)
   uint32_t by_v[2];  // 2^32 / (cap / 4) + 1 and 2^32 / (cap / 8) + 1
   float mu, omu, decay;  // omu: 1 - momentum, from 64 bits
@@ -69,7 +70,7 @@ struct Dims {
   static constexpr int BUFS = NT >= 3 ? 2 : 4;          // the warps' partial Gram matrices in shared memory at once
   static constexpr int MAT = NT * NT * 64;              // doubles of one matrix
   static constexpr int PART = TILES * 64;               // doubles of one packed upper triangle
-  static constexpr int POLY = 4 * MAT;                  // S, V and two P
+  static constexpr int POLY = (NT <= 2 ? 5 : 4) * MAT;  // S (two up to 16 rows), V and two P
   // doubles of the work space that S, V and P share with what comes before them: the warps' partial sums, then one
   // from each block of the cluster
   static constexpr int work(int cluster) {
@@ -496,6 +497,7 @@ struct Spot {
     tile_of<NT>(n, i, j);
     set(i, j);
   }
+  Spot() = default;
   __device__ __forceinline__ Spot(int i, int j) { set(i, j); }
   __device__ __forceinline__ void set(int i, int j) {
     const int lane = threadIdx.x & 31;
@@ -567,6 +569,79 @@ __device__ __forceinline__ void put_tile(double* M, const Spot<NT>& t, const dou
   }
 }
 
+// c <- the tile of S = a I + b G + c G^2 from that of G^2.
+template <int NT>
+__device__ __forceinline__ void step_form(double (&c)[2], const double2& g, const Spot<NT>& t, double ca, double cb,
+                                          double cc) {
+  const int lane = threadIdx.x & 31, r = lane >> 2, k = 2 * (lane & 3);
+  c[0] = cc * c[0] + (cb * g.x + (t.diagonal && r == k ? ca : 0.0));
+  c[1] = cc * c[1] + (cb * g.y + (t.diagonal && r == k + 1 ? ca : 0.0));
+}
+
+__device__ __forceinline__ void named_barrier(int id, int threads) {
+  asm volatile("barrier.cta.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+__device__ __forceinline__ void named_arrive(int id, int threads) {
+  asm volatile("barrier.cta.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+// The steps for up to 16 rows, where latency is all. A warp has one of the NT x NT tiles, and no mirror image to write:
+// the first half of the warps S, V and G' (the chain, which waits for itself alone), the second P', which follows with
+// two S to take from. Named barriers: 1 the chain, 2 the P warps, 3 and 4 S is there (even and odd steps), 5 and 6 S has
+// been read. At 16 x 16 a product on four warps, one to a matrix unit, takes 183 cycles with its barrier; on the three
+// tiles of a triangle with their mirror images 212, and 310 where six warps share the units.
+template <int NT>
+__device__ __forceinline__ void iterate_small(const Args& a, double* G, double* work, double inv) {
+  using D_ = Dims<NT>;
+  constexpr int T = NT * NT;
+  double *S = work, *V = work + 2 * D_::MAT, *M = work + 3 * D_::MAT;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp >= 2 * T) return;
+  const bool chain = warp < T;
+  const int n = chain ? warp : warp - T;
+  const Spot<NT> t(n / NT, n % NT);
+  double c[2];
+  if (chain) {
+    double2 g = *reinterpret_cast<const double2*>(G + t.own);
+    double sc = inv * inv;  // the first step's G still has to be scaled by it
+    for (int step = 0;; ++step) {
+      double* s = S + (step & 1) * D_::MAT;
+      const double ca = a.coef[step][0], cb = a.coef[step][1] * sc, cc = a.coef[step][2] * sc * sc;
+      product<NT>(G, G, t, c);
+      step_form(c, g, t, ca, cb, cc);
+      if (step >= 2) named_barrier(5 + (step & 1), 2 * T * 32);
+      *reinterpret_cast<double2*>(s + t.own) = make_double2(c[0], c[1]);
+      named_arrive(3 + (step & 1), 2 * T * 32);
+      if (step + 1 == a.steps) return;
+      named_barrier(1, T * 32);
+      product<NT>(s, G, t, c);
+      *reinterpret_cast<double2*>(V + t.own) = make_double2(c[0], c[1]);
+      named_barrier(1, T * 32);
+      product<NT>(s, V, t, c);
+      g = make_double2(c[0] * sc, c[1] * sc);
+      *reinterpret_cast<double2*>(G + t.own) = g;
+      named_barrier(1, T * 32);
+      sc = 1.0;
+    }
+  }
+  for (int step = 0; step < a.steps; ++step) {
+    const double* s = S + (step & 1) * D_::MAT;
+    double *from = M + ((step + 1) & 1) * D_::MAT, *to = M + (step & 1) * D_::MAT;
+    named_barrier(3 + (step & 1), 2 * T * 32);
+    if (step) {
+      product<NT>(s, from, t, c);
+    } else {
+      const double2 v = *reinterpret_cast<const double2*>(s + t.own);
+      c[0] = v.x;
+      c[1] = v.y;
+    }
+    *reinterpret_cast<double2*>(to + t.own) = make_double2(c[0], c[1]);
+    if (step + 2 < a.steps) named_arrive(5 + (step & 1), 2 * T * 32);
+    named_barrier(2, T * 32);
+  }
+}
+
 // From the Gram matrix G of x (unscaled) to P with P x = the polynomial of x, in M[0] or M[1] (returned through P). work
 // holds S, V, M[0], M[1]. Returns whether no entry of P / inv (the polynomial's own matrix) is above kMaxPlain: the
 // product with x may then be fp32, whose d roundings stay near 2^-22 of the result. Gradients of low rank have entries
@@ -578,92 +653,99 @@ __device__ bool iterate(const Args& a, double* G, double* work, double*& P) {
   double *S = work, *V = work + D_::MAT, *M = work + 2 * D_::MAT;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   double tr = 0.0;
-  for (int i = lane; i < D_::D; i += 32) tr += G[(i >> 3) * (NT + 1) * 64 + (i & 7) * 9];
+  for (int i = NT <= 2 ? lane % D_::D : lane; i < D_::D; i += 32) tr += G[(i >> 3) * (NT + 1) * 64 + (i & 7) * 9];
 #pragma unroll
-  for (int o = 16; o; o >>= 1) tr += __shfl_xor_sync(0xffffffffu, tr, o);
+  for (int o = NT == 1 ? 4 : NT == 2 ? 8 : 16; o; o >>= 1) tr += __shfl_xor_sync(0xffffffffu, tr, o);
   const double inv = 1.0 / (sqrt(tr) + a.eps);
-  // a warp's tiles: of S and of G' (R1 rounds), and of P' and V together (R2 rounds)
-  constexpr int R1 = (D_::TILES + WARPS - 1) / WARPS, R2 = (2 * D_::TILES + WARPS - 1) / WARPS;
-  double sc = inv * inv;  // the first step's G still has to be scaled by it
-  for (int step = 0; step < a.steps; ++step) {
-    const double ca = a.coef[step][0], cb = a.coef[step][1] * sc, cc = a.coef[step][2] * sc * sc;
-    const bool last = step + 1 == a.steps;
-    double *from = M + ((step + 1) & 1) * D_::MAT, *to = M + (step & 1) * D_::MAT;
-    if constexpr (NT >= 6) {
-      const int r = lane >> 2, k = 2 * (lane & 3);
-      constexpr int PARTS = WARPS / NT;  // warps of a tile row
-      const int line = warp % NT, part = warp / NT;
-      double2 row[NT];
-      if (part < PARTS) {
-        load_row<NT>(G, line, row);
-        strip<NT, PARTS>(row, G, line, part, [&](const Spot<NT>& t, double (&c)[2]) {
-          const double2 g = *reinterpret_cast<const double2*>(G + t.own);
-          c[0] = cc * c[0] + (cb * g.x + (t.diagonal && r == k ? ca : 0.0));
-          c[1] = cc * c[1] + (cb * g.y + (t.diagonal && r == k + 1 ? ca : 0.0));
-          put_tile<NT>(S, t, c);
-          if (step == 0) put_tile<NT>(to, t, c);
-        });
-      }
-      __syncthreads();
-      if (part < PARTS) {
-        load_row<NT>(S, line, row);
-        if (!last) strip<NT, PARTS>(row, G, line, part, [&](const Spot<NT>& t, double (&c)[2]) { put_tile<NT>(V, t, c); });
-        if (step) strip<NT, PARTS>(row, from, line, part, [&](const Spot<NT>& t, double (&c)[2]) { put_tile<NT>(to, t, c); });
-      }
-      if (last) break;
-      __syncthreads();
-      if (part < PARTS)
-        strip<NT, PARTS>(row, V, line, part, [&](const Spot<NT>& t, double (&c)[2]) {
-          c[0] *= sc;
-          c[1] *= sc;
-          put_tile<NT>(G, t, c);
-        });
-    } else {
+  if constexpr (2 * NT * NT <= WARPS) {
+    iterate_small<NT>(a, G, work, inv);
+    M = work + 3 * D_::MAT;
+  } else {
+    // a warp's tiles: of S and of G' (R1 rounds), and of V and P' together (R2 rounds)
+    constexpr int R1 = (D_::TILES + WARPS - 1) / WARPS, R2 = (2 * D_::TILES + WARPS - 1) / WARPS;
+    Spot<NT> chain[R1], both[R2];
+    if (NT < 6) {
 #pragma unroll
-      for (int q = 0; q < R1; ++q) {
-        const int n = warp + q * WARPS;
-        if (n < D_::TILES) {
-          const Spot<NT> t(n);
-          const double2 g = *reinterpret_cast<const double2*>(G + t.own);
-          double c[2];
-          product<NT>(G, G, t, c);
-          const int r = lane >> 2, k = 2 * (lane & 3);
-          c[0] = cc * c[0] + (cb * g.x + (t.diagonal && r == k ? ca : 0.0));
-          c[1] = cc * c[1] + (cb * g.y + (t.diagonal && r == k + 1 ? ca : 0.0));
-          put_tile<NT>(S, t, c);
-          if (step == 0) put_tile<NT>(to, t, c);
-        }
-      }
-      __syncthreads();
-      // V = S G (but in the last step) and P' = S P (from the second on), each tile by its own warp
+      for (int q = 0; q < R1; ++q) chain[q] = Spot<NT>(min(warp + q * WARPS, D_::TILES - 1));
 #pragma unroll
       for (int q = 0; q < R2; ++q) {
         const int n = warp + q * WARPS;
-        const bool isv = n < D_::TILES;
-        if (isv ? !last : n < 2 * D_::TILES && step > 0) {
-          const Spot<NT> t(isv ? n : n - D_::TILES);
-          double c[2];
-          product<NT>(S, isv ? G : from, t, c);
-          put_tile<NT>(isv ? V : to, t, c);
-        }
-      }
-      if (last) break;
-      __syncthreads();
-#pragma unroll
-      for (int q = 0; q < R1; ++q) {
-        const int n = warp + q * WARPS;
-        if (n < D_::TILES) {
-          const Spot<NT> t(n);
-          double c[2];
-          product<NT>(S, V, t, c);
-          c[0] *= sc;
-          c[1] *= sc;
-          put_tile<NT>(G, t, c);
-        }
+        both[q] = Spot<NT>(n < D_::TILES ? n : min(n - D_::TILES, D_::TILES - 1));
       }
     }
-    __syncthreads();
-    sc = 1.0;
+    double sc = inv * inv;  // the first step's G still has to be scaled by it
+    for (int step = 0; step < a.steps; ++step) {
+      const double ca = a.coef[step][0], cb = a.coef[step][1] * sc, cc = a.coef[step][2] * sc * sc;
+      const bool last = step + 1 == a.steps;
+      double *from = M + ((step + 1) & 1) * D_::MAT, *to = M + (step & 1) * D_::MAT;
+      if constexpr (NT >= 6) {
+        constexpr int PARTS = WARPS / NT;  // warps of a tile row
+        const int line = warp % NT, part = warp / NT;
+        double2 row[NT];
+        if (part < PARTS) {
+          load_row<NT>(G, line, row);
+          strip<NT, PARTS>(row, G, line, part, [&](const Spot<NT>& t, double (&c)[2]) {
+            const double2 g = *reinterpret_cast<const double2*>(G + t.own);
+            step_form(c, g, t, ca, cb, cc);
+            put_tile<NT>(S, t, c);
+            if (step == 0) put_tile<NT>(to, t, c);
+          });
+        }
+        __syncthreads();
+        if (part < PARTS) {
+          load_row<NT>(S, line, row);
+          if (!last) strip<NT, PARTS>(row, G, line, part, [&](const Spot<NT>& t, double (&c)[2]) { put_tile<NT>(V, t, c); });
+          if (step) strip<NT, PARTS>(row, from, line, part, [&](const Spot<NT>& t, double (&c)[2]) { put_tile<NT>(to, t, c); });
+        }
+        if (last) break;
+        __syncthreads();
+        if (part < PARTS)
+          strip<NT, PARTS>(row, V, line, part, [&](const Spot<NT>& t, double (&c)[2]) {
+            c[0] *= sc;
+            c[1] *= sc;
+            put_tile<NT>(G, t, c);
+          });
+      } else {
+#pragma unroll
+        for (int q = 0; q < R1; ++q) {
+          if (warp + q * WARPS < D_::TILES) {
+            const Spot<NT>& t = chain[q];
+            const double2 g = *reinterpret_cast<const double2*>(G + t.own);
+            double c[2];
+            product<NT>(G, G, t, c);
+            step_form(c, g, t, ca, cb, cc);
+            put_tile<NT>(S, t, c);
+            if (step == 0) put_tile<NT>(to, t, c);
+          }
+        }
+        __syncthreads();
+        // V = S G (but in the last step) and P' = S P (from the second on), each tile by its own warp
+#pragma unroll
+        for (int q = 0; q < R2; ++q) {
+          const int n = warp + q * WARPS;
+          const bool isv = n < D_::TILES;
+          if (isv ? !last : n < 2 * D_::TILES && step > 0) {
+            double c[2];
+            product<NT>(S, isv ? G : from, both[q], c);
+            put_tile<NT>(isv ? V : to, both[q], c);
+          }
+        }
+        if (last) break;
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < R1; ++q) {
+          if (warp + q * WARPS < D_::TILES) {
+            double c[2];
+            product<NT>(S, V, chain[q], c);
+            c[0] *= sc;
+            c[1] *= sc;
+            put_tile<NT>(G, chain[q], c);
+          }
+        }
+      }
+      __syncthreads();
+      sc = 1.0;
+    }
   }
   __syncthreads();
   P = M + ((a.steps - 1) & 1) * D_::MAT;
@@ -795,7 +877,7 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 ? 4 : 2) ortho_kernel(const 
   __shared__ __align__(8) uint64_t bar;
   double *G = sm, *work = G + D_::MAT, *slots = work + D_::BUFS * D_::PART;
   float* x = reinterpret_cast<float*>(work + D_::work(a.blocks));
-  const int rank = blockIdx.x % a.blocks, ld = pitch(a.cap);
+  const int rank = blockIdx.x & (a.blocks - 1), ld = pitch(a.cap);
   if (a.blocks > 1) {
     if (threadIdx.x == 0) {
       mbar_init(&bar, 1);
@@ -805,8 +887,8 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 ? 4 : 2) ortho_kernel(const 
     cluster_arrive();
   }
   long long base;
-  const Tensor& t = tensor_of(a, blockIdx.x / a.blocks, base);
-  const int slice = ((t.L + a.blocks - 1) / a.blocks + 7) & ~7;
+  const Tensor& t = tensor_of(a, blockIdx.x >> a.shift, base);
+  const int slice = (((t.L + a.blocks - 1) >> a.shift) + 7) & ~7;
   const int j0 = min(rank * slice, t.L), w = min(slice, t.L - j0);
 
   double acc[D_::ACC][2];
@@ -985,6 +1067,7 @@ int run_resident(Args& a, long long matrices, int maxL, cudaStream_t st) {
   int c = blocks_needed(NT, maxL);
   while (c < kMaxBlocks && maxL > 256 * c && matrices * c < 296) c *= 2;
   a.blocks = c;
+  a.shift = c == 8 ? 3 : c / 2;
   set_cap(a, ((maxL + c - 1) / c + 31) / 32 * 32);
   const long long smem = (long long)(D_::MAT + D_::work(c)) * 8 + (long long)NT * 8 * pitch(a.cap) * 4;
   return launch(ortho_kernel<NT, T, MUON>, a, matrices * c, kThreads, smem, c, st);

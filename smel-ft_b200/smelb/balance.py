@@ -38,7 +38,7 @@ def _tables(who, probs, topi, mask):
         if mask.dtype not in (torch.bool, torch.uint8) or mask.shape != (T,):
             raise _lib.SmelbError(f"{who}: mask must be bool or uint8 [{T}] (got {mask.dtype} {tuple(mask.shape)})")
         mask = mask.contiguous()
-    if probs.stride(1) != 1 or (probs.stride(0) < E and T > 1):
+    if not probs.is_contiguous() and (probs.stride(1) != 1 or (probs.stride(0) < E and T > 1)):
         probs = probs.contiguous()
     return probs, probs.stride(0), topi.contiguous(), mask
 
@@ -65,25 +65,30 @@ class _BalanceLossFn(torch.autograd.Function):
         ws = torch.empty(nb, dtype=torch.uint8, device=dev)
         _lib.call_on(dev, "smelb_balance_loss_fwd", p.data_ptr(), ld, topi.data_ptr(), _lib.ptr(mask), _lib.ptr(cu), S, T,
                      E, topi.shape[1], loss.data_ptr(), counts.data_ptr(), coef.data_ptr(), ws.data_ptr(), nb,
-                     _lib.stream_ptr(dev))
-        ctx.save_for_backward(coef, mask, cu)
-        ctx.sizes = S, T, E
+                     _lib.stream_of(dev))
+        if mask is not None or cu is not None:
+            ctx.save_for_backward(mask, cu)
+        ctx.given = mask is not None or cu is not None
+        ctx.coef, ctx.sizes = coef, (S, T, E)
         ctx.mark_non_differentiable(counts)
         ctx.set_materialize_grads(False)
         return loss, counts
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, go, _):
         if go is None:
             return None, None, None, None
-        coef, mask, cu = ctx.saved_tensors
+        if torch.is_grad_enabled():  # create_graph: the gradient depends on go, which this call would hide
+            raise _lib.SmelbError("balance_loss: there is no second derivative")
+        mask, cu = ctx.saved_tensors if ctx.given else (None, None)
         S, T, E = ctx.sizes
+        coef = ctx.coef
         dev = coef.device
-        go = go.to(device=dev, dtype=torch.float32)
+        if go.dtype != torch.float32 or go.device != dev:
+            go = go.to(device=dev, dtype=torch.float32)
         d = torch.empty(T, E, dtype=torch.float32, device=dev)
         _lib.call_on(dev, "smelb_balance_loss_bwd", coef.data_ptr(), go.data_ptr(), _lib.ptr(mask), _lib.ptr(cu), S, T, E,
-                     d.data_ptr(), _lib.stream_ptr(dev))
+                     d.data_ptr(), _lib.stream_of(dev))
         return d, None, None, None
 
 
@@ -102,23 +107,23 @@ def balance_loss(probs, topi, mask=None, cu_seqlens=None):
     return _BalanceLossFn.apply(probs, topi, mask, cu_seqlens)
 
 
-@torch.no_grad()
 def expert_usage(probs, topv, topi, mask=None):
     """(counts int64 [E], prob_mass fp32 [E], weight_mass fp32 [E]) over the rows that `mask` keeps: how often each expert
     was chosen, the sum of its probabilities and the sum of its routing weights. probs fp32 [T, E], topv bf16 or fp32
     [T, K], topi int64 [T, K], as a stats callback gets them. No gradient; the same inputs give the same bits."""
-    p, ld, i, mask = _tables("expert_usage", probs, topi, mask)
+    p, ld, i, mask = _tables("expert_usage", probs.detach() if probs.requires_grad else probs, topi, mask)
     dev = p.device
     if topv.dtype not in (torch.bfloat16, torch.float32) or topv.shape != i.shape or topv.device != dev:
         raise _lib.SmelbError(f"expert_usage: topv must be bf16 or fp32 {tuple(i.shape)} on {dev} (got {topv.dtype} "
                               f"{tuple(topv.shape)} on {topv.device})")
-    topv = topv.contiguous()
+    topv = topv.detach().contiguous() if topv.requires_grad else topv.contiguous()
     T, E = p.shape
     counts = torch.empty(E, dtype=torch.int64, device=dev)
-    mass = torch.empty(2, E, dtype=torch.float32, device=dev)
+    prob_mass = torch.empty(E, dtype=torch.float32, device=dev)
+    weight_mass = torch.empty(E, dtype=torch.float32, device=dev)
     nb = _lib.load().smelb_balance_workspace_bytes(T, E, 1, 1)
     ws = torch.empty(nb, dtype=torch.uint8, device=dev)
     _lib.call_on(dev, "smelb_expert_usage", p.data_ptr(), ld, topv.data_ptr(), 1 if topv.dtype == torch.float32 else 0,
-                 i.data_ptr(), _lib.ptr(mask), T, E, i.shape[1], counts.data_ptr(), mass.data_ptr(),
-                 mass.data_ptr() + 4 * E, ws.data_ptr(), nb, _lib.stream_ptr(dev))
-    return counts, mass[0], mass[1]
+                 i.data_ptr(), _lib.ptr(mask), T, E, i.shape[1], counts.data_ptr(), prob_mass.data_ptr(),
+                 weight_mass.data_ptr(), ws.data_ptr(), nb, _lib.stream_of(dev))
+    return counts, prob_mass, weight_mass

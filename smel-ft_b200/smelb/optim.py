@@ -8,6 +8,7 @@ The reference trains its factors with AdamW (scripts/train.py) and has no counte
 at most 64, the width of a LoRA block of the fused layer; ExpertsLoRA's [k, r, H] parameters are k matrices each.
 """
 import ctypes
+import functools
 
 import torch
 
@@ -20,16 +21,21 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 _ADJUST = {"original": 0, "match_rms_adamw": 1}
 
 
+@functools.lru_cache(maxsize=16)
+def _triples(steps, coefficients):
+    return (ctypes.c_double * (3 * steps))(*[float(v) for t in coefficients for v in t])
+
+
 def _coefficients(who, steps, coefficients):
     """Host array of 3 * steps doubles: one (a, b, c) for every step, or a triple of its own for each."""
-    if not 1 <= int(steps) <= MAX_STEPS:
+    if not 1 <= steps <= MAX_STEPS:
         raise _lib.SmelbError(f"{who}: {steps} steps (1..{MAX_STEPS})")
-    c = list(coefficients)
-    if len(c) == 3 and not any(hasattr(v, "__len__") for v in c):
-        c = [c] * steps
+    c = tuple(coefficients)
+    if len(c) == 3 and not hasattr(c[0], "__len__"):
+        c = (c,) * steps
     if len(c) != steps or any(not hasattr(t, "__len__") or len(t) != 3 for t in c):
         raise _lib.SmelbError(f"{who}: coefficients are three numbers, or three for each of the {steps} steps")
-    return (ctypes.c_double * (3 * steps))(*[float(v) for t in c for v in t])
+    return _triples(steps, tuple(map(tuple, c)))
 
 
 def _matrices(who, t, what):
@@ -57,18 +63,18 @@ def orthogonalize(x, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
     batch, m, n = _matrices("orthogonalize", x, "x")
     if not eps > 0:
         raise _lib.SmelbError("orthogonalize: eps must be positive")
+    steps = int(steps)
     c = _coefficients("orthogonalize", steps, coefficients)
     x = x.contiguous()
     out = torch.empty_like(x)
     if batch:
         nb = _lib.load().smelb_orthogonalize_workspace_bytes(batch, m, n)
         ws = torch.empty(nb, dtype=torch.uint8, device=x.device) if nb > 0 else None
-        _lib.call_on(x.device, "smelb_orthogonalize", x.data_ptr(), _DTYPES[x.dtype], batch, m, n, int(steps), c,
-                     float(eps), out.data_ptr(), _lib.ptr(ws), nb, _lib.stream_ptr(x.device))
+        _lib.call_on(x.device, "smelb_orthogonalize", x.data_ptr(), _DTYPES[x.dtype], batch, m, n, steps, c,
+                     float(eps), out.data_ptr(), _lib.ptr(ws), nb, _lib.stream_of(x.device))
     return out
 
 
-@torch.no_grad()
 def muon_step(params, grads, buffers, lr, momentum=0.95, nesterov=True, weight_decay=0.0, adjust="original", steps=5,
               coefficients=COEFFICIENTS, eps=1e-7):
     """One Muon update of the tensors params[i] with the gradients grads[i] and momentum buffers buffers[i], in place:
@@ -88,34 +94,47 @@ def muon_step(params, grads, buffers, lr, momentum=0.95, nesterov=True, weight_d
         raise _lib.SmelbError(f"{who}: adjust must be one of {sorted(_ADJUST)}")
     if not eps > 0:
         raise _lib.SmelbError(f"{who}: eps must be positive")
+    steps = int(steps)
     c = _coefficients(who, steps, coefficients)
     if not params:
         return
     dev, dtype = params[0].device, params[0].dtype
-    table = (_lib.MuonTensor * len(params))()
-    keep = []
+    if not params[0].is_cuda or dtype not in _DTYPES:
+        _matrices(who, params[0], "params[0]")  # says which it is
+    on, fp32 = dev.index, torch.float32
+    rows, keep = [], []
     for i, (p, g, m) in enumerate(zip(params, grads, buffers)):
-        batch, rows, cols = _matrices(who, p, f"params[{i}]")
-        if p.dtype != dtype or p.device != dev:
-            raise _lib.SmelbError(f"{who}: params[{i}] is {p.dtype} on {p.device}, params[0] {dtype} on {dev}")
-        if g.dtype != dtype or g.device != dev or g.shape != p.shape:
-            raise _lib.SmelbError(f"{who}: grads[{i}] is {g.dtype} {tuple(g.shape)} on {g.device}, its parameter {dtype} "
-                                  f"{tuple(p.shape)} on {dev}")
-        if m.dtype != torch.float32 or m.device != dev or m.shape != p.shape:
-            raise _lib.SmelbError(f"{who}: buffers[{i}] must be fp32 {tuple(p.shape)} on {dev} (got {m.dtype} "
-                                  f"{tuple(m.shape)} on {m.device})")
-        if not (p.is_contiguous() and m.is_contiguous()):
-            raise _lib.SmelbError(f"{who}: params[{i}] and buffers[{i}] must be contiguous (they are updated in place)")
+        shape = p.shape
+        if not (p.dtype is dtype and g.dtype is dtype and m.dtype is fp32 and g.shape == shape and m.shape == shape and
+                p.get_device() == on and g.get_device() == on and m.get_device() == on and len(shape) >= 2 and
+                1 <= min(shape[-2:]) <= MAX_SHORT_SIDE and p.is_contiguous() and m.is_contiguous()):
+            _refuse(who, i, p, g, m, dtype, dev)
         if not g.is_contiguous():
             g = g.contiguous()
             keep.append(g)
-        t = table[i]
-        t.p, t.g, t.m, t.batch, t.rows, t.cols = p.data_ptr(), g.data_ptr(), m.data_ptr(), batch, rows, cols
+        rows += (p.data_ptr(), g.data_ptr(), m.data_ptr(), p.numel() // (shape[-1] * shape[-2]), shape[-2], shape[-1])
+    # the fields of a MuonTensor are eight bytes each: an array of integers is an array of them
+    table = (ctypes.c_int64 * len(rows))(*rows)
     nb = _lib.load().smelb_muon_workspace_bytes(table, len(params))
     ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb > 0 else None
     _lib.call_on(dev, "smelb_muon_step", table, len(params), _DTYPES[dtype], float(lr), float(momentum),
-                 1 if nesterov else 0, float(weight_decay), _ADJUST[adjust], int(steps), c, float(eps), _lib.ptr(ws), nb,
-                 _lib.stream_ptr(dev))
+                 1 if nesterov else 0, float(weight_decay), _ADJUST[adjust], steps, c, float(eps), _lib.ptr(ws), nb,
+                 _lib.stream_of(dev))
+    torch.autograd.graph.increment_version(params + buffers)  # as torch's in-place operations do
+
+
+def _refuse(who, i, p, g, m, dtype, dev):
+    """Says what is wrong with tensor i of a step."""
+    _matrices(who, p, f"params[{i}]")
+    if p.dtype != dtype or p.device != dev:
+        raise _lib.SmelbError(f"{who}: params[{i}] is {p.dtype} on {p.device}, params[0] {dtype} on {dev}")
+    if g.dtype != dtype or g.device != dev or g.shape != p.shape:
+        raise _lib.SmelbError(f"{who}: grads[{i}] is {g.dtype} {tuple(g.shape)} on {g.device}, its parameter {dtype} "
+                              f"{tuple(p.shape)} on {dev}")
+    if m.dtype != torch.float32 or m.device != dev or m.shape != p.shape:
+        raise _lib.SmelbError(f"{who}: buffers[{i}] must be fp32 {tuple(p.shape)} on {dev} (got {m.dtype} "
+                              f"{tuple(m.shape)} on {m.device})")
+    raise _lib.SmelbError(f"{who}: params[{i}] and buffers[{i}] must be contiguous (they are updated in place)")
 
 
 class Muon(torch.optim.Optimizer):

@@ -257,6 +257,15 @@ def test_gradient_against_differences(dev):
     assert abs((a.double() - b.double()) - want) <= 2 * 131 * U * (a.double() + b.double())
 
 
+def test_no_second_derivative(dev):
+    import smelb
+    probs, topi, _, _ = routing(dev, 20, 8, 2, 8)
+    p = probs.clone().requires_grad_(True)
+    loss = smelb.balance_loss(p, topi)[0]
+    with pytest.raises(smelb.SmelbError, match="second derivative"):
+        torch.autograd.grad(loss, p, create_graph=True)
+
+
 def test_through_the_layer(dev, golden):
     """moe_forward with the loss taken in its stats callback, as a training step uses it: dx and the usage against the
     oracle in 64 bits with the same choices, and a no-loss step as before."""

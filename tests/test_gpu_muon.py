@@ -237,6 +237,16 @@ def test_unaligned_and_noncontiguous_gradients(dev):
         assert torch.equal(p, q) and torch.equal(m, n)
 
 
+def test_a_backward_over_changed_parameters_is_refused(dev):
+    """The step changes params in place, and autograd notices as after any in-place operation."""
+    import smelb
+    p = torch.randn(16, 64, device=dev, requires_grad=True)
+    y = (p * p).sum()
+    smelb.muon_step([p], [torch.randn(16, 64, device=dev)], [torch.zeros(16, 64, device=dev)], lr=0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
 def test_streams_and_graphs(dev):
     """On another stream, captured twice and replayed at once: each replay moves its own tensors one step."""
     import smelb

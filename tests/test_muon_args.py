@@ -31,6 +31,9 @@ class _Fake:
     def data_ptr(self):
         return 1 << 20
 
+    def get_device(self):
+        return self.device.index
+
 
 @pytest.mark.parametrize("t,text", [(_Fake((16,)), "matrices"), (_Fake((16, 32), torch.float16), "matrices"),
                                     (_Fake((65, 65)), "short side"), (_Fake((2, 0, 4)), "short side"),
