@@ -425,7 +425,7 @@ int smelb_lm_logits(const void* h, int64_t N, int64_t H, const void* w, const vo
  * choices of e and P[s][e] the sum of their probs[.][e]:
  *   loss (fp32 [1]) = 1/S' sum_s E / (K n_s^2) sum_e c[s][e] P[s][e] over the S' sequences with n_s > 0 (0 without any)
  *   counts (int64 [S][E]) = c;  coef (fp32 [S * E + 1]): the gradient's rows, for smelb_balance_loss_bwd.
- * Rows outside every sequence and rows the mask drops are not read and have a zero gradient. Indices outside [0, E)
+ * Rows outside every sequence and rows the mask drops may hold anything and have a zero gradient. Indices outside [0, E)
  * are not counted and recorded in the status word. E <= 512, K <= 32. workspace: 256-byte aligned,
  * smelb_balance_workspace_bytes(T, E, S, 0) bytes. Equal inputs give equal bits. */
 int64_t smelb_balance_workspace_bytes(int64_t T, int64_t E, int64_t S, int usage);

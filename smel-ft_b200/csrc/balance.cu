@@ -25,7 +25,10 @@ constexpr int kTileThreads = 512;
 constexpr int kTileWarps = kTileThreads / 32;
 constexpr int kMaxTileRows = 128;
 constexpr int kMaxE = 512, kMaxK = 32;
-constexpr int kFinCols = 32, kFinLanes = 32;
+// A finishing block adds COLS experts of one sequence with kFinThreads / COLS threads each: 32 where sequences are many, 8
+// where the records of few of them are long lists (one sequence of 65537 rows and 128 experts, 586 records: 16 us in four
+// blocks of 32 experts).
+constexpr int kFinThreads = 512;
 
 struct TileArgs {
   const float* probs;
@@ -36,6 +39,7 @@ struct TileArgs {
   const uint8_t* mask;
   const int* cu;
   int S, E, K, rows;
+  uint32_t by_k;  // 2^32 / K + 1 (K > 1)
   long long T;
   float* rec_mass;    // [records][E]
   float* rec_weight;  // [records][E], usage only
@@ -55,6 +59,8 @@ __device__ __forceinline__ void seq_range(const int* cu, int s, long long T, lon
   }
 }
 
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
 // Number of sequences that end at or before row t: the first one that can hold it. Called by the whole block.
 __device__ __forceinline__ int first_seq(const int* cu, int S, long long t) {
   int s0 = 0;
@@ -67,7 +73,7 @@ __device__ __forceinline__ int first_seq(const int* cu, int S, long long t) {
 }
 
 template <int VEC, bool USAGE>
-__global__ void __launch_bounds__(kTileThreads) balance_tile_kernel(const TileArgs a) {
+__global__ void __launch_bounds__(kTileThreads, USAGE ? 4 : 3) balance_tile_kernel(const TileArgs a) {
   __shared__ uint8_t ok[kMaxTileRows];
   __shared__ int cnt[kMaxE];
   __shared__ float red[kTileThreads * VEC];
@@ -75,6 +81,13 @@ __global__ void __launch_bounds__(kTileThreads) balance_tile_kernel(const TileAr
   const int tid = threadIdx.x, E = a.E, K = a.K;
   const long long t0 = (long long)blockIdx.x * a.rows;
   const int rows = (int)min((long long)a.rows, a.T - t0);
+  // the tile's rows are on their way to L2 while the block finds out which of them count
+  if (a.ld == E) {
+    const char* p = reinterpret_cast<const char*>(a.probs + t0 * E);
+    for (int b = tid * 128; b < rows * E * 4; b += kTileThreads * 128) prefetch_l2(p + b);
+  }
+  for (int b = tid * 128; b < rows * K * 8; b += kTileThreads * 128)
+    prefetch_l2(reinterpret_cast<const char*>(a.topi + t0 * K) + b);
   if (blockIdx.x == 0 && tid == 0) *a.ticket = 0;
   if (tid < rows) ok[tid] = a.mask ? a.mask[t0 + tid] != 0 : 1;
   const int ncol = (E + VEC - 1) / VEC, lanes = kTileThreads / ncol;
@@ -96,7 +109,7 @@ __global__ void __launch_bounds__(kTileThreads) balance_tile_kernel(const TileAr
     for (int base = i0; base < i1; base += kTileThreads) {
       const int i = base + tid;
       int e = -1;
-      if (i < i1 && ok[i / K]) {
+      if (i < i1 && ok[K == 1 ? i : (int)__umulhi((uint32_t)i, a.by_k)]) {
         const long long v = a.topi[t0 * K + i];
         if (v >= 0 && v < E) {
           e = (int)v;
@@ -124,19 +137,29 @@ __global__ void __launch_bounds__(kTileThreads) balance_tile_kernel(const TileAr
 #pragma unroll
     for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
     if (lane < lanes) {
+      // U rows in flight; a row that does not count is read and left out (its values may be anything)
+      constexpr int U = 4;
       const float* p = a.probs + t0 * a.ld + col;
-#pragma unroll 4
-      for (int r = ra + lane; r < rb; r += lanes) {
-        if (ok[r]) {
-          if (VEC == 4) {
-            const float4 v = __ldg(reinterpret_cast<const float4*>(p + r * a.ld));
-            acc[0] += v.x;
-            acc[1 % VEC] += v.y;
-            acc[2 % VEC] += v.z;
-            acc[3 % VEC] += v.w;
+      for (int r = ra + lane; r < rb; r += U * lanes) {
+        float v[U][VEC];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int q = min(r + u * lanes, rb - 1);
+          if constexpr (VEC == 4) {
+            const float4 f = __ldg(reinterpret_cast<const float4*>(p + q * a.ld));
+            v[u][0] = f.x;
+            v[u][1] = f.y;
+            v[u][2] = f.z;
+            v[u][3] = f.w;
           } else {
-            acc[0] += __ldg(p + r * a.ld);
+            v[u][0] = __ldg(p + q * a.ld);
           }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const bool counts = r + u * lanes < rb && ok[min(r + u * lanes, rb - 1)];
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) acc[j] += counts ? v[u][j] : 0.f;
         }
       }
 #pragma unroll
@@ -175,15 +198,16 @@ struct FinArgs {
   int* ticket;
 };
 
-template <bool USAGE>
-__global__ void __launch_bounds__(kFinCols* kFinLanes) balance_finish_kernel(const FinArgs a) {
-  __shared__ double sm[kFinLanes][kFinCols + 1];
-  __shared__ double sw[USAGE ? kFinLanes : 1][kFinCols + 1];
-  __shared__ int sc[kFinLanes][kFinCols + 1];
-  __shared__ int sn[kFinLanes];
-  __shared__ int last;
-  const int s = blockIdx.x, col = threadIdx.x & 31, lane = threadIdx.x >> 5, E = a.E;
-  const int e = blockIdx.y * kFinCols + col;
+template <bool USAGE, int COLS>
+__global__ void __launch_bounds__(kFinThreads) balance_finish_kernel(const FinArgs a) {
+  constexpr int LANES = kFinThreads / COLS, WARPS = kFinThreads / 32;
+  __shared__ double sm[LANES][COLS + 1];
+  __shared__ double sw[USAGE ? LANES : 1][COLS + 1];
+  __shared__ int sc[LANES][COLS + 1];
+  __shared__ int sn[LANES];
+  __shared__ bool last;
+  const int s = blockIdx.x, col = threadIdx.x % COLS, lane = threadIdx.x / COLS, E = a.E;
+  const int e = blockIdx.y * COLS + col;
   long long lo, hi;
   seq_range(a.cu, s, a.T, lo, hi);
   double m = 0.0, w = 0.0;
@@ -191,7 +215,7 @@ __global__ void __launch_bounds__(kFinCols* kFinLanes) balance_finish_kernel(con
   if (lo < hi) {
     const int b1 = (int)((hi - 1) / a.rows);
 #pragma unroll 4
-    for (int b = (int)(lo / a.rows) + lane; b <= b1; b += kFinLanes) {
+    for (int b = (int)(lo / a.rows) + lane; b <= b1; b += LANES) {
       const long long rec = (long long)b + s;
       n += a.rec_n[rec];
       if (e < E) {
@@ -206,18 +230,26 @@ __global__ void __launch_bounds__(kFinCols* kFinLanes) balance_finish_kernel(con
   if (USAGE) sw[lane][col] = w;
   if (col == 0) sn[lane] = n;
   __syncthreads();
-  if (lane == 0) {
+  // the first warp adds the lanes' sums: 32 / COLS threads to a column, then across them
+  if (threadIdx.x < 32) {
     m = w = 0.0;
     long long cs = 0, ns = 0;
 #pragma unroll 8
-    for (int l = 0; l < kFinLanes; ++l) {
+    for (int l = lane; l < LANES; l += 32 / COLS) {
       m += sm[l][col];
       cs += sc[l][col];
       ns += sn[l];
       if (USAGE) w += sw[l][col];
     }
+#pragma unroll
+    for (int o = 16; o >= COLS; o >>= 1) {
+      m += __shfl_xor_sync(0xffffffffu, m, o);
+      cs += __shfl_xor_sync(0xffffffffu, cs, o);
+      ns += __shfl_xor_sync(0xffffffffu, ns, o);
+      if (USAGE) w += __shfl_xor_sync(0xffffffffu, w, o);
+    }
     double part = 0.0;
-    if (e < E) {
+    if (e < E && lane == 0) {
       a.counts[(long long)s * E + e] = cs;
       if (USAGE) {
         a.prob_mass[e] = (float)m;
@@ -231,7 +263,7 @@ __global__ void __launch_bounds__(kFinCols* kFinLanes) balance_finish_kernel(con
     if (!USAGE) {
 #pragma unroll
       for (int o = 16; o; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
-      if (col == 0) {
+      if (threadIdx.x == 0) {
         a.part[(long long)s * gridDim.y + blockIdx.y] = part;
         if (blockIdx.y == 0) a.seq_n[s] = (int)min(ns, 1LL);
         __threadfence();
@@ -248,23 +280,24 @@ __global__ void __launch_bounds__(kFinCols* kFinLanes) balance_finish_kernel(con
   const volatile int* seqs = a.seq_n;
   double sum = 0.0;
   int some = 0;
-  for (long long i = threadIdx.x; i < (long long)gridDim.x * gridDim.y; i += blockDim.x) sum += parts[i];
-  for (int i = threadIdx.x; i < a.S; i += blockDim.x) some += seqs[i];
+  for (long long i = threadIdx.x; i < (long long)gridDim.x * gridDim.y; i += kFinThreads) sum += parts[i];
+  for (int i = threadIdx.x; i < a.S; i += kFinThreads) some += seqs[i];
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
     sum += __shfl_xor_sync(0xffffffffu, sum, o);
     some += __shfl_xor_sync(0xffffffffu, some, o);
   }
-  if (col == 0) {
-    sm[lane][0] = sum;
-    sn[lane] = some;
+  double* ws = &sm[0][0];
+  if (threadIdx.x % 32 == 0) {
+    ws[threadIdx.x / 32] = sum;
+    sn[threadIdx.x / 32] = some;
   }
   __syncthreads();
   if (threadIdx.x == 0) {
     sum = 0.0;
     some = 0;
-    for (int l = 0; l < kFinLanes; ++l) {
-      sum += sm[l][0];
+    for (int l = 0; l < WARPS; ++l) {
+      sum += ws[l];
       some += sn[l];
     }
     const double inv = 1.0 / max(some, 1);
@@ -324,13 +357,15 @@ int tile_rows(long long T) {
 struct Layout {
   long long mass, weight, cnt, n, part, seq_n, ticket, total;
   int rows, tiles;
+  int cols;  // experts of a finishing block
 };
 
 Layout layout(long long T, long long E, long long S, bool usage) {
   Layout l{};
   l.rows = tile_rows(T);
   l.tiles = (int)((T + l.rows - 1) / l.rows);
-  const long long recs = l.tiles + S, eb = (E + kFinCols - 1) / kFinCols;
+  l.cols = S * E < 32 * 148 ? 8 : 32;
+  const long long recs = l.tiles + S, eb = (E + l.cols - 1) / l.cols;
   long long o = 0;
   auto take = [&](long long bytes) {
     const long long at = o;
@@ -355,6 +390,9 @@ int check_sizes(const char* what, int64_t T, int64_t E, int64_t K, int64_t S) {
   return kOk;
 }
 
+// Factor of the division of a tile's choice by K.
+uint32_t by(int64_t K) { return (uint32_t)((1ull << 32) / K + 1); }
+
 template <bool USAGE>
 int run_tiles(const TileArgs& t, int tiles, cudaStream_t st) {
   if (!tiles) return kOk;
@@ -362,6 +400,16 @@ int run_tiles(const TileArgs& t, int tiles, cudaStream_t st) {
   const size_t smem = USAGE ? (size_t)kTileWarps * t.E * sizeof(float) : 0;
   if (vec) balance_tile_kernel<4, USAGE><<<tiles, kTileThreads, smem, st>>>(t);
   else balance_tile_kernel<1, USAGE><<<tiles, kTileThreads, smem, st>>>(t);
+  SMELB_CUDA(cudaGetLastError());
+  count_launch();
+  return kOk;
+}
+
+template <bool USAGE>
+int run_finish(const FinArgs& f, int cols, cudaStream_t st) {
+  const dim3 grid((unsigned)f.S, (unsigned)((f.E + cols - 1) / cols));
+  if (cols == 8) balance_finish_kernel<USAGE, 8><<<grid, kFinThreads, 0, st>>>(f);
+  else balance_finish_kernel<USAGE, 32><<<grid, kFinThreads, 0, st>>>(f);
   SMELB_CUDA(cudaGetLastError());
   count_launch();
   return kOk;
@@ -398,18 +446,14 @@ int smelb_balance_loss_fwd(const float* probs, int64_t ld, const int64_t* topi, 
   cudaStream_t st = (cudaStream_t)stream;
   int* ticket = (int*)(ws + l.ticket);
   if (l.tiles == 0) SMELB_CUDA(cudaMemsetAsync(ticket, 0, sizeof(int), st));
-  const TileArgs t{probs, ld, (const long long*)topi, nullptr, 0, mask, cu_seqlens, (int)S, (int)E, (int)K, l.rows, T,
+  const TileArgs t{probs, ld, (const long long*)topi, nullptr, 0, mask, cu_seqlens, (int)S, (int)E, (int)K, l.rows, by(K), T,
                    (float*)(ws + l.mass), nullptr, (int*)(ws + l.cnt), (int*)(ws + l.n), ticket,
                    device_status_on(dev, st)};
   if (int rc = run_tiles<false>(t, l.tiles, st)) return rc;
   const FinArgs f{t.rec_mass, nullptr, t.rec_cnt, t.rec_n, cu_seqlens, (int)S, (int)E, (int)K, l.rows, T,
                   (long long*)counts, coef, loss, nullptr, nullptr, (double*)(ws + l.part), (int*)(ws + l.seq_n),
                   ticket};
-  balance_finish_kernel<false><<<dim3((unsigned)S, (unsigned)((E + kFinCols - 1) / kFinCols)), kFinCols * kFinLanes, 0,
-                                 st>>>(f);
-  SMELB_CUDA(cudaGetLastError());
-  count_launch();
-  return kOk;
+  return run_finish<false>(f, l.cols, st);
 }
 
 int smelb_balance_loss_bwd(const float* coef, const float* go, const uint8_t* mask, const int32_t* cu_seqlens,
@@ -445,16 +489,13 @@ int smelb_expert_usage(const float* probs, int64_t ld, const void* topv, int top
   SMELB_CUDA(cudaGetDevice(&dev));
   char* ws = (char*)workspace;
   cudaStream_t st = (cudaStream_t)stream;
-  const TileArgs t{probs, ld, (const long long*)topi, topv, topv_fp32, mask, nullptr, 1, (int)E, (int)K, l.rows, T,
+  const TileArgs t{probs, ld, (const long long*)topi, topv, topv_fp32, mask, nullptr, 1, (int)E, (int)K, l.rows, by(K), T,
                    (float*)(ws + l.mass), (float*)(ws + l.weight), (int*)(ws + l.cnt), (int*)(ws + l.n),
                    (int*)(ws + l.ticket), device_status_on(dev, st)};
   if (int rc = run_tiles<true>(t, l.tiles, st)) return rc;
   const FinArgs f{t.rec_mass, t.rec_weight, t.rec_cnt, t.rec_n, nullptr, 1, (int)E, (int)K, l.rows, T,
                   (long long*)counts, nullptr, nullptr, prob_mass, weight_mass, nullptr, nullptr, nullptr};
-  balance_finish_kernel<true><<<dim3(1, (unsigned)((E + kFinCols - 1) / kFinCols)), kFinCols * kFinLanes, 0, st>>>(f);
-  SMELB_CUDA(cudaGetLastError());
-  count_launch();
-  return kOk;
+  return run_finish<true>(f, l.cols, st);
 }
 
 }  // extern "C"

@@ -100,7 +100,7 @@ def balance_loss(probs, topi, mask=None, cu_seqlens=None):
     which is 1 for uniform probabilities; the loss is 0 when no row is kept. cu_seqlens (int32 [S + 1], not decreasing, on
     the device) gives sequence s the rows cu_seqlens[s] .. cu_seqlens[s + 1] - 1 (empty ones allowed) and counts the
     shape [S, E]; without it all rows are one sequence and counts has the shape [E]. Rows outside every sequence and rows
-    that the mask drops are not read (they may hold anything) and get a zero gradient.
+    that the mask drops may hold anything and get a zero gradient.
 
     Differentiable w.r.t. probs, with the counts as constants; the same inputs give the same bits. Choices outside [0, E)
     are not counted and recorded in the status word (read_status)."""
