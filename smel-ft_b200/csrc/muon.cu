@@ -42,6 +42,7 @@ struct Tensor {
 struct Args {
   Tensor t[kMaxTensors];
   int n, steps;
+  long long first;   // split: the launch's first matrix
   int blocks;        // blocks of one matrix; resident: a power of two, 2^shift
   int shift;
   int cap;           // columns that a block holds at once (a multiple of 32)
@@ -940,7 +941,7 @@ __global__ void __launch_bounds__(kThreads, NT == 6 || MUON || sizeof(T) == 2 ? 
   float* x = reinterpret_cast<float*>(work + D_::BUFS * D_::PART);
   const int block = blockIdx.x % a.blocks, ld = pitch(a.cap), warp = threadIdx.x >> 5;
   long long base;
-  const Tensor& t = tensor_of(a, blockIdx.x / a.blocks, base);
+  const Tensor& t = tensor_of(a, a.first + blockIdx.x / a.blocks, base);
   double acc[D_::ACC][2];
 #pragma unroll
   for (int n = 0; n < D_::ACC; ++n) acc[n][0] = acc[n][1] = 0.0;
@@ -992,7 +993,7 @@ __global__ void __launch_bounds__(kThreads, NT >= 6 && !MUON && sizeof(T) == 4 ?
   const int block = blockIdx.x % a.blocks, ld = pitch(a.cap);
   const long long mat = blockIdx.x / a.blocks;
   long long base;
-  const Tensor& t = tensor_of(a, mat, base);
+  const Tensor& t = tensor_of(a, a.first + mat, base);
   const double* form = a.form + mat * (D_::MAT + 2);
   const bool plain = form[D_::MAT] != 0.0;
   if (plain) round_form<NT>(form, reinterpret_cast<float*>(sm));
@@ -1050,13 +1051,18 @@ int blocks_needed(int nt, int L) {
   return c;
 }
 
+static_assert(sizeof(Args) <= 4096, "kernel parameters");
 static_assert(kSplitCap <= kThreads * 2 / 4, "apply_plain takes a chunk at once from 48 rows on");
+
+// Matrices of one round of the split way: their partial Gram matrices and P are the workspace (50 KB each at 64 rows).
+constexpr long long kSplitRound = 4096;
 
 // Blocks for one matrix of the split way: as many chunks to each as leave eight blocks for an SM, and at most two blocks on
 // every SM for one matrix (their partial Gram matrices are added by one block).
 int split_blocks(long long matrices, int L) {
   const long long chunks = (L + kSplitCap - 1) / kSplitCap;
-  const long long per = std::max({1LL, chunks * matrices / (148 * 8), (chunks + 295) / 296});
+  const long long per =
+      std::max({1LL, chunks * std::min(matrices, kSplitRound) / (148 * 8), (chunks + 295) / 296});
   return (int)((chunks + per - 1) / per);
 }
 
@@ -1078,13 +1084,20 @@ int run_split(Args& a, long long matrices, int maxL, double* ws, cudaStream_t st
   using D_ = Dims<NT>;
   a.blocks = split_blocks(matrices, maxL);
   set_cap(a, kSplitCap);
-  a.gram = ws;
-  a.form = ws + matrices * a.blocks * D_::PART;
   const long long x = (long long)NT * 8 * pitch(a.cap) * 4;
-  int rc = launch(gram_kernel<NT, T, MUON>, a, matrices * a.blocks, kThreads, (long long)D_::BUFS * D_::PART * 8 + x, 1, st);
-  if (rc == kOk) rc = launch(form_kernel<NT>, a, matrices, form_warps<NT>() * 32, (long long)(D_::MAT + D_::POLY) * 8, 1, st);
-  if (rc == kOk) rc = launch(product_kernel<NT, T, MUON>, a, matrices * a.blocks, kThreads, (long long)D_::MAT * 8 + x, 1, st);
-  return rc;
+  const int blocks = a.blocks;
+  for (a.first = 0; a.first < matrices; a.first += kSplitRound) {
+    const long long n = std::min(kSplitRound, matrices - a.first);
+    a.gram = ws;
+    a.form = ws + n * blocks * D_::PART;
+    if (int rc = launch(gram_kernel<NT, T, MUON>, a, n * blocks, kThreads, (long long)D_::BUFS * D_::PART * 8 + x, 1, st))
+      return rc;
+    if (int rc = launch(form_kernel<NT>, a, n, form_warps<NT>() * 32, (long long)(D_::MAT + D_::POLY) * 8, 1, st))
+      return rc;
+    if (int rc = launch(product_kernel<NT, T, MUON>, a, n * blocks, kThreads, (long long)D_::MAT * 8 + x, 1, st))
+      return rc;
+  }
+  return kOk;
 }
 
 template <int NT, typename T, bool MUON>
@@ -1171,7 +1184,7 @@ long long workspace(const smelb_muon_tensor* t, int64_t n) {
   for_launches(t, n, [&](int nt, bool held, const int64_t*, int, long long matrices, int maxL) {
     if (!held) {
       const long long part = nt * (nt + 1) / 2 * 64, form = nt * nt * 64 + 2;
-      most = std::max(most, matrices * (split_blocks(matrices, maxL) * part + form) * 8);
+      most = std::max(most, std::min(matrices, kSplitRound) * (split_blocks(matrices, maxL) * part + form) * 8);
     }
     return 0;
   });

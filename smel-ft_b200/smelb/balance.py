@@ -20,6 +20,22 @@ from . import _lib
 
 def _tables(who, probs, topi, mask):
     """Checked routing tables: (probs with unit column stride, its row pitch, topi, mask as bytes)."""
+    ps, ts = probs.shape, topi.shape
+    ok = (probs.is_cuda and topi.is_cuda and probs.dtype is torch.float32 and topi.dtype is torch.int64 and
+          len(ps) == 2 and len(ts) == 2 and ts[0] == ps[0] and 1 <= ps[1] <= 512 and 1 <= ts[1] <= 32 and
+          probs.get_device() == topi.get_device())
+    if mask is not None:
+        ok = (ok and mask.is_cuda and mask.get_device() == probs.get_device() and mask.shape == ps[:1] and
+              (mask.dtype is torch.bool or mask.dtype is torch.uint8))
+    if not ok:
+        _refuse(who, probs, topi, mask)
+    if not probs.is_contiguous() and (probs.stride(1) != 1 or (probs.stride(0) < ps[1] and ps[0] > 1)):
+        probs = probs.contiguous()
+    return probs, probs.stride(0), topi.contiguous(), None if mask is None else mask.contiguous()
+
+
+def _refuse(who, probs, topi, mask):
+    """Says what is wrong with the tables."""
     for name, t in (("probs", probs), ("topi", topi), ("mask", mask)):
         if t is None and name == "mask":
             continue
@@ -34,13 +50,7 @@ def _tables(who, probs, topi, mask):
         raise _lib.SmelbError(f"{who}: topi must be int64 [{T}, K] (got {topi.dtype} {tuple(topi.shape)})")
     if not 1 <= E <= 512 or not 1 <= topi.shape[1] <= 32:
         raise _lib.SmelbError(f"{who}: E={E} (1..512) and K={topi.shape[1]} (1..32)")
-    if mask is not None:
-        if mask.dtype not in (torch.bool, torch.uint8) or mask.shape != (T,):
-            raise _lib.SmelbError(f"{who}: mask must be bool or uint8 [{T}] (got {mask.dtype} {tuple(mask.shape)})")
-        mask = mask.contiguous()
-    if not probs.is_contiguous() and (probs.stride(1) != 1 or (probs.stride(0) < E and T > 1)):
-        probs = probs.contiguous()
-    return probs, probs.stride(0), topi.contiguous(), mask
+    raise _lib.SmelbError(f"{who}: mask must be bool or uint8 [{T}] (got {mask.dtype} {tuple(mask.shape)})")
 
 
 class _BalanceLossFn(torch.autograd.Function):

@@ -101,18 +101,25 @@ def muon_step(params, grads, buffers, lr, momentum=0.95, nesterov=True, weight_d
     dev, dtype = params[0].device, params[0].dtype
     if not params[0].is_cuda or dtype not in _DTYPES:
         _matrices(who, params[0], "params[0]")  # says which it is
-    on, fp32 = dev.index, torch.float32
+    on, fp32, most = dev.index, torch.float32, MAX_SHORT_SIDE
     rows, keep = [], []
     for i, (p, g, m) in enumerate(zip(params, grads, buffers)):
         shape = p.shape
-        if not (p.dtype is dtype and g.dtype is dtype and m.dtype is fp32 and g.shape == shape and m.shape == shape and
-                p.get_device() == on and g.get_device() == on and m.get_device() == on and len(shape) >= 2 and
-                1 <= min(shape[-2:]) <= MAX_SHORT_SIDE and p.is_contiguous() and m.is_contiguous()):
+        if not (p.dtype is dtype and g.dtype is dtype and m.dtype is fp32 and g.shape == shape == m.shape and
+                p.get_device() == g.get_device() == m.get_device() == on and len(shape) >= 2 and
+                p.is_contiguous() and m.is_contiguous()):
+            _refuse(who, i, p, g, m, dtype, dev)
+        a, b = shape[-2], shape[-1]
+        if not (a > 0 and b > 0 and (a <= most or b <= most)):
             _refuse(who, i, p, g, m, dtype, dev)
         if not g.is_contiguous():
             g = g.contiguous()
             keep.append(g)
-        rows += (p.data_ptr(), g.data_ptr(), m.data_ptr(), p.numel() // (shape[-1] * shape[-2]), shape[-2], shape[-1])
+        rows += (p.data_ptr(), g.data_ptr(), m.data_ptr(), p.numel() // (a * b), a, b)
+    written = [q for q in rows[0::6] + rows[2::6] if q]
+    once = set(written)
+    if len(once) < len(written) or not once.isdisjoint(rows[1::6]):
+        raise _lib.SmelbError(f"{who}: a tensor is given twice")
     # the fields of a MuonTensor are eight bytes each: an array of integers is an array of them
     table = (ctypes.c_int64 * len(rows))(*rows)
     nb = _lib.load().smelb_muon_workspace_bytes(table, len(params))
@@ -120,7 +127,8 @@ def muon_step(params, grads, buffers, lr, momentum=0.95, nesterov=True, weight_d
     _lib.call_on(dev, "smelb_muon_step", table, len(params), _DTYPES[dtype], float(lr), float(momentum),
                  1 if nesterov else 0, float(weight_decay), _ADJUST[adjust], steps, c, float(eps), _lib.ptr(ws), nb,
                  _lib.stream_of(dev))
-    torch.autograd.graph.increment_version(params + buffers)  # as torch's in-place operations do
+    # as torch's in-place operations do
+    torch.autograd.graph.increment_version([t for t in params + buffers if not t.is_inference()])
 
 
 def _refuse(who, i, p, g, m, dtype, dev):

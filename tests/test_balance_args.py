@@ -21,6 +21,9 @@ class _Fake:
     def dim(self):
         return len(self.shape)
 
+    def get_device(self):
+        return self.device.index
+
 
 @pytest.mark.parametrize("probs,topi,mask,text", [
     (((4, 8), torch.bfloat16), ((4, 2), torch.int64), None, "fp32"),

@@ -104,6 +104,8 @@ def test_balance_loss_nothing_kept(dev):
     check(dev, probs, topi, part, torch.tensor([0, 50, 100], dtype=torch.int32, device=dev))
     loss, counts = smelb.balance_loss(probs[:0], topi[:0])
     assert loss.item() == 0 and counts.sum().item() == 0
+    loss, counts = smelb.balance_loss(probs[:0], topi[:0], None, torch.zeros(4, dtype=torch.int32, device=dev))
+    assert loss.item() == 0 and counts.shape == (3, 32) and not counts.any()
     p = probs[:0].detach().requires_grad_(True)
     smelb.balance_loss(p, topi[:0])[0].backward()
     assert p.grad.shape == (0, 32)

@@ -89,7 +89,8 @@ def test_orthogonalize(dev, m, n, dtype):
     assert torch.equal(out, smelb.orthogonalize(x))
 
 
-@pytest.mark.parametrize("batch,m,n", [(1, 16, 2048), (300, 16, 512), (700, 512, 16), (150, 64, 300), (0, 16, 64), (1000, 2, 3)])
+@pytest.mark.parametrize("batch,m,n", [(1, 16, 2048), (300, 16, 512), (700, 512, 16), (150, 64, 300), (0, 16, 64), (1000, 2, 3),
+                                       (4100, 33, 34), (5000, 8, 16)])
 def test_orthogonalize_batches(dev, batch, m, n):
     import smelb
     x = matrices(dev, (batch, m, n), "full", batch)

@@ -15,7 +15,8 @@ def test_cpu_tensors_are_refused():
 
 
 class _Fake:
-    def __init__(self, shape, dtype=torch.float32, device="cuda:0"):
+    def __init__(self, shape, dtype=torch.float32, device="cuda:0", at=1 << 20):
+        self.at = at
         self.shape, self.dtype, self.device, self.is_cuda = torch.Size(shape), dtype, torch.device(device), True
         self.requires_grad = False
 
@@ -29,7 +30,7 @@ class _Fake:
         return self.shape[-1] != 99
 
     def data_ptr(self):
-        return 1 << 20
+        return self.at
 
     def get_device(self):
         return self.device.index
@@ -69,6 +70,11 @@ def test_tensors_that_do_not_fit_together():
                           ([ok, _Fake((2, 16, 32), torch.bfloat16)], [ok, ok], [ok, ok], "params"),
                           ([_Fake((16, 99))], [_Fake((16, 99))], [_Fake((16, 99))], "contiguous")):
         with pytest.raises(smelb.SmelbError, match=text):
+            smelb.muon_step(p, g, m, lr=0.1)
+    a, b, c = (_Fake((2, 16, 32), at=k << 20) for k in (1, 2, 3))
+    for p, g, m in (([a], [b], [a]), ([a, a], [b, b], [c, _Fake((2, 16, 32), at=5 << 20)]), ([a], [a], [b]),
+                    ([a], [c], [c]), ([a, b], [c, c], [_Fake((2, 16, 32), at=7 << 20)] * 2)):
+        with pytest.raises(smelb.SmelbError, match="twice"):
             smelb.muon_step(p, g, m, lr=0.1)
     with pytest.raises(smelb.SmelbError, match="adjust"):
         smelb.muon_step([ok], [ok], [ok], lr=0.1, adjust="rms")
@@ -124,6 +130,7 @@ def test_workspace_sizes():
     assert ws(12, 16, 2048) == 0 and ws(12, 2048, 16) == 0 and ws(5, 32, 2816) == 0 and ws(0, 64, 2048) == 0
     assert ws(5, 32, 2817) > 0 and ws(1, 16, 4097) > 0 and ws(1, 33, 40) > 0
     assert ws(1000, 64, 2048) >= 1000 * (36 + 64) * 64 * 8 and ws(1, 64, 1 << 20) >= 256 * 36 * 64 * 8
+    assert ws(1 << 20, 64, 64) == ws(4096, 64, 64)  # rounds of 4096 matrices
     assert ws(1, 65, 65) == -1 and ws(-1, 16, 16) == -1
     t = (_lib.MuonTensor * 2)()
     for i, (b, m, n) in enumerate(((3, 64, 500), (7, 2000, 48))):
