@@ -35,7 +35,8 @@ struct Tensor {
   long long start;  // matrices before this tensor's
   int d, L;         // short and long side
   int tall;         // memory is [L][d] (else [d][L])
-  uint32_t by_d;    // 2^32 / d + 1: division by d
+  // factors of divisions, 2^32 / n + 1: by d, and by the columns that kThreads vectors of 4 or 8 elements cover at once
+  uint32_t by_d, by_jump[2];
   float step;       // lr * shape factor
 };
 
@@ -46,7 +47,10 @@ struct Args {
   int blocks;        // blocks of one matrix; resident: a power of two, 2^shift
   int shift;
   int cap;           // columns that a block holds at once (a multiple of 32)
-  uint32_t by_v[2];  // 2^32 / (cap / 4) + 1 and 2^32 / (cap / 8) + 1
+  // wide matrices in vectors of 4 and 8 elements: the rows that the block covers at once (two or more: cap is at most 512),
+  // and the factors of divisions by the vectors of a row and by those rows
+  int rows[2];
+  uint32_t by_v[2], by_rows[2];
   float mu, omu, decay;  // omu: 1 - momentum, from 64 bits
   int nesterov;
   double eps;
@@ -147,65 +151,53 @@ __device__ __forceinline__ uint4 repack(const Vec<bf16>& o) {
 }
 
 
-// The vectors of N elements of a block's columns [j0, j0 + w): vector q of a wide matrix is row q / (cap / N), columns from
-// N (q % (cap / N)); a tall matrix is contiguous, element e of it is (i, j) = (e % d, e / d).
-template <int N, bool TALL>
-struct Place {
-  int i, j;
-  bool live;
-  __device__ __forceinline__ Place(const Args& a, const Tensor& t, int w, int q) {
-    if (TALL) {
-      j = (int)__umulhi((uint32_t)(q * N), t.by_d);
-      i = q * N - j * t.d;
-      live = j < w;
+// A thread's vectors of N elements among a block's columns [j0, j0 + w). Its place along the contiguous side is fixed and
+// it goes along the other one, so that a vector costs two additions: in a wide matrix [d][L] the thread has the columns
+// from N (tid % (cap / N)) of every rows-th row, in a tall one [L][d] N of the d elements of every columns-th column.
+template <int N>
+struct Walk {
+  int n;            // vectors
+  int at, step;     // offset in memory from (0, j0), and to the next vector (a matrix has less than 2^31 elements)
+  int in, in_step;  // the same in x
+  __device__ __forceinline__ Walk(const Args& a, const Tensor& t, int w, int ld) {
+    const int tid = threadIdx.x;
+    if (t.tall) {
+      const int j = (int)__umulhi((uint32_t)(tid * N), t.by_d), i = tid * N - j * t.d;
+      const int jump = (int)__umulhi((uint32_t)(kThreads * N), t.by_d);  // columns that the block covers at once
+      n = j < jump && j < w ? (int)__umulhi((uint32_t)(w - 1 - j), t.by_jump[N == 8]) + 1 : 0;
+      at = tid * N;
+      step = jump * t.d;
+      in = i * ld + j;
+      in_step = jump;
     } else {
-      i = (int)__umulhi((uint32_t)q, a.by_v[N == 8]);
-      j = (q - i * (a.cap / N)) * N;
-      live = i < t.d && j < w;
+      const int i = (int)__umulhi((uint32_t)tid, a.by_v[N == 8]), j = (tid - i * (a.cap / N)) * N;
+      const int jump = a.rows[N == 8];  // rows that the block covers at once
+      n = i < jump && i < t.d && j < w ? (int)__umulhi((uint32_t)(t.d - 1 - i), a.by_rows[N == 8]) + 1 : 0;
+      at = i * t.L + j;
+      step = jump * t.L;
+      in = i * ld + j;
+      in_step = jump * ld;
     }
   }
-  // offset in memory from column j0
-  __device__ __forceinline__ long long at(const Tensor& t) const {
-    return TALL ? (long long)(j * t.d + i) : (long long)i * t.L + j;
-  }
 };
-template <int N>
-__device__ __forceinline__ int places(const Args& a, const Tensor& t, int w) {
-  return t.tall ? w * t.d / N : t.d * (a.cap / N);
-}
 
 // The N elements of a vector: v -> x (PUT) or x -> v.
 template <bool PUT, int N, bool TALL>
-__device__ __forceinline__ void move(const Tensor& t, const Place<N, TALL>& at, float* x, int ld, float (&v)[N]) {
+__device__ __forceinline__ void move(float* c, int ld, float (&v)[N]) {
   if (TALL) {
-    float* c = x + at.i * ld + at.j;
-    if (t.d % N == 0) {
-#pragma unroll
-      for (int k = 0; k < N; ++k) {
-        if (PUT) c[k * ld] = v[k];
-        else v[k] = c[k * ld];
-      }
-      return;
-    }
-    int i = at.i;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-      if (PUT) *c = v[k];
-      else v[k] = *c;
-      c += ld;
-      if (++i == t.d) {
-        i = 0;
-        c += 1 - t.d * ld;
-      }
+      if (PUT) c[k * ld] = v[k];
+      else v[k] = c[k * ld];
     }
   } else {
 #pragma unroll
     for (int k = 0; k < N; k += 4) {
-      float4* c = reinterpret_cast<float4*>(x + at.i * ld + at.j + k);
+      float4* f = reinterpret_cast<float4*>(c + k);
       if (PUT) {
-        *c = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+        *f = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
       } else {
-        const float4 o = *c;
+        const float4 o = *f;
         v[k] = o.x;
         v[k + 1] = o.y;
         v[k + 2] = o.z;
@@ -221,31 +213,31 @@ __device__ __forceinline__ bool vectors(const Tensor& t, long long base, int w) 
   constexpr int N = 16 / sizeof(T);
   const uintptr_t at = (uintptr_t)(reinterpret_cast<const T*>(t.g) + base) |
                        (uintptr_t)(reinterpret_cast<T*>(t.p) + base) | (MUON ? (uintptr_t)(t.m + base) : 0);
-  return (at & 15) == 0 && (t.tall ? (w * t.d) % N == 0 : t.L % N == 0 && w % N == 0);
+  return (at & 15) == 0 && (t.tall ? t.d % N == 0 : t.L % N == 0 && w % N == 0);
 }
 
 template <typename T, bool MUON, bool TALL>
 __device__ __forceinline__ void load_vectors(const Args& a, const Tensor& t, const T* g, float* m, int w, float* x,
                                              int ld, bool first) {
   constexpr int N = Vec<T>::N, U = MUON && N == 8 ? 2 : 4;  // vectors in flight per thread
-  const int end = places<N>(a, t, w);
-  for (int q0 = threadIdx.x; q0 < end; q0 += kThreads * U) {
+  const Walk<N> walk(a, t, w, ld);
+  int at = walk.at;
+  float* in = x + walk.in;
+  for (int left = walk.n; left > 0; left -= U) {
     uint4 rg[U], rm[U][N / 4];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const Place<N, TALL> at(a, t, w, q0 + u * kThreads);
-      if (at.live) {
-        rg[u] = __ldg(reinterpret_cast<const uint4*>(g + at.at(t)));
+      if (u < left) {
+        rg[u] = __ldg(reinterpret_cast<const uint4*>(g + at + u * walk.step));
         if (MUON) {
 #pragma unroll
-          for (int k = 0; k < N / 4; ++k) rm[u][k] = *reinterpret_cast<const uint4*>(m + at.at(t) + 4 * k);
+          for (int k = 0; k < N / 4; ++k) rm[u][k] = *reinterpret_cast<const uint4*>(m + at + u * walk.step + 4 * k);
         }
       }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const Place<N, TALL> at(a, t, w, q0 + u * kThreads);
-      if (at.live) {
+      if (u < left) {
         Vec<T> v;
         unpack(rg[u], v);
         if (MUON) {
@@ -255,13 +247,27 @@ __device__ __forceinline__ void load_vectors(const Args& a, const Tensor& t, con
             unpack(rm[u][k], b);
 #pragma unroll
             for (int l = 0; l < 4; ++l) v.v[4 * k + l] = update(a, v.v[4 * k + l], b.v[l], first);
-            if (first) *reinterpret_cast<uint4*>(m + at.at(t) + 4 * k) = repack(b);
+            if (first) *reinterpret_cast<uint4*>(m + at + u * walk.step + 4 * k) = repack(b);
           }
         }
-        move<true>(t, at, x, ld, v.v);
+        move<true, N, TALL>(in + u * walk.in_step, ld, v.v);
       }
     }
+    at += U * walk.step;
+    in += U * walk.in_step;
   }
+}
+
+// Element q of columns [j0, j0 + w): its place in x and its offset in memory from (0, j0).
+__device__ __forceinline__ int element_at(const Tensor& t, int w, int q, int& i, int& j) {
+  if (t.tall) {
+    j = q / t.d;
+    i = q - j * t.d;
+    return q;
+  }
+  i = q / w;
+  j = q - i * w;
+  return i * t.L + j;
 }
 
 // Columns [j0, j0 + w) (j0 a multiple of 8) into x, zeros up to the next multiple of 8 and in the rows that fill the
@@ -279,8 +285,8 @@ __device__ __forceinline__ void load_slice(const Args& a, const Tensor& t, long 
     load_vectors<T, MUON, false>(a, t, g, m, w, x, ld, first);
   } else {
     for (int q = threadIdx.x; q < w * t.d; q += kThreads) {
-      const int i = t.tall ? q % t.d : q / w, j = t.tall ? q / t.d : q % w;
-      const long long at = t.tall ? (long long)q : (long long)i * t.L + j;
+      int i, j;
+      const int at = element_at(t, w, q, i, j);
       float v = to_f(g[at]);
       if (MUON) {
         float b = m[at];
@@ -310,28 +316,29 @@ __device__ __forceinline__ float result(const Args& a, const Tensor& t, float o,
 template <typename T, bool MUON, bool TALL>
 __device__ __forceinline__ void store_vectors(const Args& a, const Tensor& t, T* p, int w, float* x, int ld) {
   constexpr int N = Vec<T>::N, U = 4;
-  const int end = places<N>(a, t, w);
-  for (int q0 = threadIdx.x; q0 < end; q0 += kThreads * U) {
+  const Walk<N> walk(a, t, w, ld);
+  int at = walk.at;
+  float* in = x + walk.in;
+  for (int left = walk.n; left > 0; left -= U) {
     uint4 rp[U];
     if (MUON) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const Place<N, TALL> at(a, t, w, q0 + u * kThreads);
-        if (at.live) rp[u] = *reinterpret_cast<const uint4*>(p + at.at(t));
-      }
+      for (int u = 0; u < U; ++u)
+        if (u < left) rp[u] = *reinterpret_cast<const uint4*>(p + at + u * walk.step);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const Place<N, TALL> at(a, t, w, q0 + u * kThreads);
-      if (at.live) {
+      if (u < left) {
         Vec<T> v, was{};
         if (MUON) unpack(rp[u], was);
-        move<false>(t, at, x, ld, v.v);
+        move<false, N, TALL>(in + u * walk.in_step, ld, v.v);
 #pragma unroll
         for (int k = 0; k < N; ++k) v.v[k] = result<MUON>(a, t, v.v[k], was.v[k]);
-        *reinterpret_cast<uint4*>(p + at.at(t)) = repack(v);
+        *reinterpret_cast<uint4*>(p + at + u * walk.step) = repack(v);
       }
     }
+    at += U * walk.step;
+    in += U * walk.in_step;
   }
 }
 
@@ -347,8 +354,8 @@ __device__ __forceinline__ void store_slice(const Args& a, const Tensor& t, long
     store_vectors<T, MUON, false>(a, t, p, w, x, ld);
   } else {
     for (int q = threadIdx.x; q < w * t.d; q += kThreads) {
-      const int i = t.tall ? q % t.d : q / w, j = t.tall ? q / t.d : q % w;
-      T* at = p + (t.tall ? (long long)q : (long long)i * t.L + j);
+      int i, j;
+      T* at = p + element_at(t, w, q, i, j);
       put(at, result<MUON>(a, t, x[i * ld + j], MUON ? to_f(*at) : 0.f));
     }
   }
@@ -1011,10 +1018,17 @@ __global__ void __launch_bounds__(kThreads, NT >= 6 && !MUON && sizeof(T) == 4 ?
   }
 }
 
+// Factor of a division of a number below 2^16 by n > 1: the high word of the product is the quotient.
+uint32_t by(int n) { return (uint32_t)((1ull << 32) / n + 1); }
+
 void set_cap(Args& a, int cap) {
   a.cap = cap;
-  a.by_v[0] = (uint32_t)((1ull << 32) / (cap / 4) + 1);
-  a.by_v[1] = (uint32_t)((1ull << 32) / (cap / 8) + 1);
+  for (int k = 0; k < 2; ++k) {
+    const int vectors = cap / (k ? 8 : 4);
+    a.rows[k] = kThreads / vectors;
+    a.by_v[k] = by(vectors);
+    a.by_rows[k] = by(a.rows[k]);
+  }
 }
 
 template <typename F>
@@ -1227,8 +1241,8 @@ int run(const smelb_muon_tensor* t, int64_t n, int dtype, bool muon, double lr, 
       const int d = (int)std::min(s.rows, s.cols), L = (int)std::max(s.rows, s.cols);
       const double f = adjust == 1 ? 0.2 * sqrt((double)L) : sqrt(std::max(1.0, (double)s.rows / (double)s.cols));
       // a single column is a single row in memory
-      a.t[k] = Tensor{s.p, s.g, s.m, start, d, L, s.rows > s.cols && d > 1 ? 1 : 0, (uint32_t)((1ull << 32) / d + 1),
-                      (float)(lr * f)};
+      a.t[k] = Tensor{s.p, s.g, s.m, start, d, L, s.rows > s.cols && d > 1 ? 1 : 0, by(d),
+                      {by(kThreads * 4 / d), by(kThreads * 8 / d)}, (float)(lr * f)};
       start += s.batch;
     }
     const bool bf = dtype == 1;
