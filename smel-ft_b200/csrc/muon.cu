@@ -32,7 +32,9 @@ struct Tensor {
   void* p;          // parameter (momentum step) or output
   const void* g;    // gradient or input
   float* m;         // momentum buffer
-  long long start;  // matrices before this tensor's
+  long long start;  // split: matrices before this tensor's; resident: clusters
+  int batch;        // matrices
+  int shift;        // resident: 2^shift blocks of a cluster hold one matrix
   int d, L;         // short and long side
   int tall;         // memory is [L][d] (else [d][L])
   // factors of divisions, 2^32 / n + 1: by d, and by the columns that kThreads vectors of 4 or 8 elements cover at once
@@ -44,7 +46,7 @@ struct Args {
   Tensor t[kMaxTensors];
   int n, steps;
   long long first;   // split: the launch's first matrix
-  int blocks;        // blocks of one matrix; resident: a power of two, 2^shift
+  int blocks;        // split: blocks of one matrix; resident: of a cluster, 2^shift
   int shift;
   int cap;           // columns that a block holds at once (a multiple of 32)
   // wide matrices in vectors of 4 and 8 elements: the rows that the block covers at once (two or more: cap is at most 512),
@@ -863,19 +865,18 @@ __device__ __forceinline__ void apply_plain(const float* Pf, float* x, int ld, i
   }
 }
 
-// The tensor of matrix `mat` and its first element.
-__device__ __forceinline__ const Tensor& tensor_of(const Args& a, long long mat, long long& base) {
+// The tensor that unit `at` (see Tensor::start) belongs to.
+__device__ __forceinline__ const Tensor& tensor_of(const Args& a, long long at) {
   int ti = 0;
   for (int end = a.n; end - ti > 1;) {
     const int mid = (ti + end) / 2;
-    if (a.t[mid].start <= mat) ti = mid;
+    if (a.t[mid].start <= at) ti = mid;
     else end = mid;
   }
-  base = (mat - a.t[ti].start) * (long long)a.t[ti].d * a.t[ti].L;
   return a.t[ti];
 }
 
-// Resident: the blocks of a cluster hold one matrix, `cap` columns each at most. Their parts of the Gram matrix go to every
+// Resident: the blocks of a cluster hold one matrix, or a few short ones, `cap` columns each at most. Their parts of the Gram matrix go to every
 // block's shared memory by asynchronous stores that the receiver's barrier counts: one way, and without the fence over
 // the stores to the momentum buffer that a cluster barrier would need.
 template <int NT, typename T, bool MUON>
@@ -885,18 +886,29 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 ? 4 : 2) ortho_kernel(const 
   __shared__ __align__(8) uint64_t bar;
   double *G = sm, *work = G + D_::MAT, *slots = work + D_::BUFS * D_::PART;
   float* x = reinterpret_cast<float*>(work + D_::work(a.blocks));
-  const int rank = blockIdx.x & (a.blocks - 1), ld = pitch(a.cap);
+  const Tensor& t = tensor_of(a, blockIdx.x >> a.shift);
+  // the blocks of this block's matrix: from `first` in the cluster, `rank` among them
+  const int place = blockIdx.x & (a.blocks - 1), blocks = 1 << t.shift, rank = place & (blocks - 1), first = place - rank;
+  const int ld = pitch(a.cap);
   if (a.blocks > 1) {
-    if (threadIdx.x == 0) {
+    if (threadIdx.x == 0 && blocks > 1) {
       mbar_init(&bar, 1);
       fence_mbar_init();
-      mbar_arrive_expect_tx(&bar, (uint32_t)(a.blocks * D_::PART * sizeof(double)));
+      mbar_arrive_expect_tx(&bar, (uint32_t)(blocks * D_::PART * sizeof(double)));
     }
     cluster_arrive();
   }
-  long long base;
-  const Tensor& t = tensor_of(a, blockIdx.x >> a.shift, base);
-  const int slice = (((t.L + a.blocks - 1) >> a.shift) + 7) & ~7;
+  const long long matrix = (((blockIdx.x >> a.shift) - t.start) << (a.shift - t.shift)) + (place >> t.shift);
+  if (matrix >= t.batch) {  // the last cluster of a tensor is not full
+    if (a.blocks > 1) {
+      cluster_wait();
+      cluster_arrive_relaxed();
+      cluster_wait();
+    }
+    return;
+  }
+  const long long base = matrix * t.d * t.L;
+  const int slice = (((t.L + blocks - 1) >> t.shift) + 7) & ~7;
   const int j0 = min(rank * slice, t.L), w = min(slice, t.L - j0);
 
   double acc[D_::ACC][2];
@@ -905,25 +917,25 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 ? 4 : 2) ortho_kernel(const 
   if (w) load_slice<NT, T, MUON>(a, t, base, j0, w, x, ld, true);
   __syncthreads();
   gram<NT, 0>(x, ld, w, threadIdx.x >> 5, acc);
-  if (a.blocks > 1) {
-    cluster_wait();  // every block's barrier is set up
+  if (a.blocks > 1) cluster_wait();  // every block's barrier is set up
+  if (blocks > 1) {
     reduce_warps<NT>(acc, work, [&](int q, double v0, double v1) {
-      for (int r = 0; r < a.blocks; ++r) push(slots + rank * D_::PART + q, &bar, r, v0, v1);
+      for (int r = 0; r < blocks; ++r) push(slots + rank * D_::PART + q, &bar, first + r, v0, v1);
     });
     mbar_wait(&bar, 0, a.err, kDevErrWaitCluster, blockIdx.x);
     for (int q = threadIdx.x; q < D_::PART; q += kThreads) {
       double s = 0.0;
 #pragma unroll 4
-      for (int r = 0; r < a.blocks; ++r) s += slots[r * D_::PART + q];
+      for (int r = 0; r < blocks; ++r) s += slots[r * D_::PART + q];
       spread<NT>(G, q, s);
     }
-    cluster_arrive_relaxed();  // for the exit: this block's pushes are under way
   } else {
     reduce_warps<NT>(acc, work, [&](int q, double v0, double v1) {
       spread<NT>(G, q, v0);
       spread<NT>(G, q + 1, v1);
     });
   }
+  if (a.blocks > 1) cluster_arrive_relaxed();  // for the exit: this block's pushes are under way
   __syncthreads();
   double* P;
   if (iterate<NT, kWarps>(a, G, work, P)) {
@@ -947,8 +959,9 @@ __global__ void __launch_bounds__(kThreads, NT == 6 || MUON || sizeof(T) == 2 ? 
   double* work = sm;
   float* x = reinterpret_cast<float*>(work + D_::BUFS * D_::PART);
   const int block = blockIdx.x % a.blocks, ld = pitch(a.cap), warp = threadIdx.x >> 5;
-  long long base;
-  const Tensor& t = tensor_of(a, a.first + blockIdx.x / a.blocks, base);
+  const long long mat = a.first + blockIdx.x / a.blocks;
+  const Tensor& t = tensor_of(a, mat);
+  const long long base = (mat - t.start) * t.d * t.L;
   double acc[D_::ACC][2];
 #pragma unroll
   for (int n = 0; n < D_::ACC; ++n) acc[n][0] = acc[n][1] = 0.0;
@@ -999,8 +1012,8 @@ __global__ void __launch_bounds__(kThreads, NT >= 6 && !MUON && sizeof(T) == 4 ?
   float* x = reinterpret_cast<float*>(sm + D_::MAT);
   const int block = blockIdx.x % a.blocks, ld = pitch(a.cap);
   const long long mat = blockIdx.x / a.blocks;
-  long long base;
-  const Tensor& t = tensor_of(a, a.first + mat, base);
+  const Tensor& t = tensor_of(a, a.first + mat);
+  const long long base = (a.first + mat - t.start) * t.d * t.L;
   const double* form = a.form + mat * (D_::MAT + 2);
   const bool plain = form[D_::MAT] != 0.0;
   if (plain) round_form<NT>(form, reinterpret_cast<float*>(sm));
@@ -1080,17 +1093,31 @@ int split_blocks(long long matrices, int L) {
   return (int)((chunks + per - 1) / per);
 }
 
+int log2_of(int c) { return c == 8 ? 3 : c / 2; }
+
 template <int NT, typename T, bool MUON>
 int run_resident(Args& a, long long matrices, int maxL, cudaStream_t st) {
   using D_ = Dims<NT>;
-  // few matrices: more blocks for each, down to 256 columns, until two are on every SM
+  // few matrices: more blocks for each, down to 256 columns, until two are on every SM, and the same for all. Many: each
+  // as many as it needs, short ones side by side in a cluster (a short matrix spread over the blocks of a long one would
+  // form P in each of them, and a launch of its own would leave SMs idle at its end).
   int c = blocks_needed(NT, maxL);
-  while (c < kMaxBlocks && maxL > 256 * c && matrices * c < 296) c *= 2;
+  const bool few = matrices * c <= 148 * 4;
+  while (few && c < kMaxBlocks && maxL > 256 * c && matrices * c < 296) c *= 2;
   a.blocks = c;
-  a.shift = c == 8 ? 3 : c / 2;
-  set_cap(a, ((maxL + c - 1) / c + 31) / 32 * 32);
+  a.shift = log2_of(c);
+  long long clusters = 0;
+  int cap = 32;
+  for (int k = 0; k < a.n; ++k) {
+    Tensor& t = a.t[k];
+    t.shift = few ? a.shift : log2_of(blocks_needed(NT, t.L));
+    t.start = clusters;
+    clusters += (t.batch + (c >> t.shift) - 1) >> (a.shift - t.shift);
+    cap = std::max(cap, (((t.L + (1 << t.shift) - 1) >> t.shift) + 31) / 32 * 32);
+  }
+  set_cap(a, cap);
   const long long smem = (long long)(D_::MAT + D_::work(c)) * 8 + (long long)NT * 8 * pitch(a.cap) * 4;
-  return launch(ortho_kernel<NT, T, MUON>, a, matrices * c, kThreads, smem, c, st);
+  return launch(ortho_kernel<NT, T, MUON>, a, clusters * c, kThreads, smem, c, st);
 }
 
 template <int NT, typename T, bool MUON>
@@ -1149,46 +1176,29 @@ int check_shapes(const smelb_muon_tensor* t, int64_t n, const char* what) {
 }
 
 // Calls f(row tiles, held, the launch's tensors idx[0 .. count), matrices, longest side) for every launch: tensors of the
-// same row tiles and way, at most kMaxTensors. Resident matrices that fill the SMs more than once go by the blocks that
-// they need (a short matrix spread over the blocks of a long one forms P in each of them); fewer take one launch.
+// same row tiles and way, at most kMaxTensors.
 template <typename F>
 int for_launches(const smelb_muon_tensor* t, int64_t n, F&& f) {
-  for (int nt : kTileCounts) {
-    long long held = 0;
-    bool any = false;
-    int most = 1;
-    for (int64_t i = 0; i < n; ++i) {
-      const int d = (int)std::min(t[i].rows, t[i].cols), L = (int)std::max(t[i].rows, t[i].cols);
-      if (t[i].batch == 0 || tiles_for(d) != nt) continue;
-      any = true;
-      if (resident(nt, L)) {
-        held += t[i].batch;
-        most = std::max(most, blocks_needed(nt, L));
-      }
-    }
-    if (!any) continue;
-    const bool apart = held * most > 148 * 4;
-    for (int way = 0; way <= kMaxBlocks; way = way ? 2 * way : 1) {  // 0: split; else blocks of a resident matrix
+  for (int nt : kTileCounts)
+    for (int held = 0; held < 2; ++held) {
       int64_t idx[kMaxTensors];
       int count = 0, maxL = 0;
       long long matrices = 0;
       for (int64_t i = 0; i < n; ++i) {
         const int d = (int)std::min(t[i].rows, t[i].cols), L = (int)std::max(t[i].rows, t[i].cols);
-        if (t[i].batch == 0 || tiles_for(d) != nt) continue;
-        if (way != (!resident(nt, L) ? 0 : apart ? blocks_needed(nt, L) : 1)) continue;
+        if (t[i].batch == 0 || tiles_for(d) != nt || resident(nt, L) != (held != 0)) continue;
         idx[count++] = i;
         matrices += t[i].batch;
         maxL = std::max(maxL, L);
         if (count == kMaxTensors) {
-          if (int rc = f(nt, way != 0, idx, count, matrices, maxL)) return rc;
+          if (int rc = f(nt, held != 0, idx, count, matrices, maxL)) return rc;
           count = maxL = 0;
           matrices = 0;
         }
       }
       if (count)
-        if (int rc = f(nt, way != 0, idx, count, matrices, maxL)) return rc;
+        if (int rc = f(nt, held != 0, idx, count, matrices, maxL)) return rc;
     }
-  }
   return kOk;
 }
 
@@ -1241,7 +1251,7 @@ int run(const smelb_muon_tensor* t, int64_t n, int dtype, bool muon, double lr, 
       const int d = (int)std::min(s.rows, s.cols), L = (int)std::max(s.rows, s.cols);
       const double f = adjust == 1 ? 0.2 * sqrt((double)L) : sqrt(std::max(1.0, (double)s.rows / (double)s.cols));
       // a single column is a single row in memory
-      a.t[k] = Tensor{s.p, s.g, s.m, start, d, L, s.rows > s.cols && d > 1 ? 1 : 0, by(d),
+      a.t[k] = Tensor{s.p, s.g, s.m, start, (int)s.batch, 0, d, L, s.rows > s.cols && d > 1 ? 1 : 0, by(d),
                       {by(kThreads * 4 / d), by(kThreads * 8 / d)}, (float)(lr * f)};
       start += s.batch;
     }

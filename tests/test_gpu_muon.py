@@ -210,6 +210,22 @@ def test_muon_step(dev, options, dtype):
     check_step(before, params, grads, bufs, 0.02, **o)
 
 
+@pytest.mark.parametrize("shapes", [
+    [(301, 16, 2048), (333, 16, 512), (7, 1000, 16), (1, 16, 30), (50, 513, 12)],
+    [(101, 32, 2816), (51, 352, 32), (3, 32, 353), (1, 25, 25), (90, 25, 705)],
+    [(150, 8, 4096), (1, 2000, 8), (5, 7, 600), (601, 8, 8)],
+])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_muon_step_long_and_short_matrices(dev, shapes, dtype):
+    """Enough matrices that short ones share a cluster: batches that do not fill their last one, one to eight blocks for a
+    matrix."""
+    import smelb
+    params, grads, bufs = tensors(dev, shapes, 5, dtype)
+    before = [(p.clone(), m.clone()) for p, m in zip(params, bufs)]
+    smelb.muon_step(params, grads, bufs, lr=0.02, weight_decay=0.1)
+    check_step(before, params, grads, bufs, 0.02, wd=0.1)
+
+
 def test_muon_step_many_tensors(dev):
     """More tensors than one launch takes, and long ones that a block reads twice."""
     import smelb
