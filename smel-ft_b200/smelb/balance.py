@@ -53,41 +53,36 @@ def _refuse(who, probs, topi, mask):
     raise _lib.SmelbError(f"{who}: mask must be bool or uint8 [{T}] (got {mask.dtype} {tuple(mask.shape)})")
 
 
+def _loss(p, ld, topi, mask, cu, counts):
+    """The loss and its gradient's rows; fills counts."""
+    dev = p.device
+    T, E = p.shape
+    S = 1 if cu is None else cu.numel() - 1
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    coef = torch.empty(S * E + 1, dtype=torch.float32, device=dev)
+    nb = _lib.load().smelb_balance_workspace_bytes(T, E, S, 0)
+    ws = torch.empty(nb, dtype=torch.uint8, device=dev)
+    _lib.call_on(dev, "smelb_balance_loss_fwd", p.data_ptr(), ld, topi.data_ptr(), _lib.ptr(mask), _lib.ptr(cu), S, T, E,
+                 topi.shape[1], loss.data_ptr(), counts.data_ptr(), coef.data_ptr(), ws.data_ptr(), nb,
+                 _lib.stream_of(dev))
+    return loss, coef, (S, T, E)
+
+
 class _BalanceLossFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, probs, topi, mask, cu):
-        p, ld, topi, mask = _tables("balance_loss", probs, topi, mask)
-        dev = p.device
-        T, E = p.shape
-        S = 1
-        if cu is not None:
-            if not cu.is_cuda or cu.device != dev:
-                raise _lib.SmelbError(f"balance_loss: cu_seqlens on {cu.device}, probs on {dev}")
-            if cu.dtype != torch.int32 or cu.dim() != 1 or cu.numel() < 2:
-                raise _lib.SmelbError(f"balance_loss: cu_seqlens must be int32 [sequences + 1] (got {cu.dtype} "
-                                      f"{tuple(cu.shape)})")
-            cu = cu.contiguous()
-            S = cu.numel() - 1
-        loss = torch.empty((), dtype=torch.float32, device=dev)
-        counts = torch.empty((E,) if cu is None else (S, E), dtype=torch.int64, device=dev)
-        coef = torch.empty(S * E + 1, dtype=torch.float32, device=dev)
-        nb = _lib.load().smelb_balance_workspace_bytes(T, E, S, 0)
-        ws = torch.empty(nb, dtype=torch.uint8, device=dev)
-        _lib.call_on(dev, "smelb_balance_loss_fwd", p.data_ptr(), ld, topi.data_ptr(), _lib.ptr(mask), _lib.ptr(cu), S, T,
-                     E, topi.shape[1], loss.data_ptr(), counts.data_ptr(), coef.data_ptr(), ws.data_ptr(), nb,
-                     _lib.stream_of(dev))
-        if mask is not None or cu is not None:
-            ctx.save_for_backward(mask, cu)
-        ctx.given = mask is not None or cu is not None
-        ctx.coef, ctx.sizes = coef, (S, T, E)
-        ctx.mark_non_differentiable(counts)
-        ctx.set_materialize_grads(False)
-        return loss, counts
+    """The loss alone, of probs and the checked tables as one object: autograd's time on the host grows with the inputs and
+    outputs it sees."""
 
     @staticmethod
-    def backward(ctx, go, _):
-        if go is None:
-            return None, None, None, None
+    def forward(ctx, probs, tables):
+        loss, ctx.coef, ctx.sizes = _loss(*tables)
+        mask, cu = tables[3:5]
+        ctx.given = mask is not None or cu is not None
+        if ctx.given:
+            ctx.save_for_backward(mask, cu)
+        return loss
+
+    @staticmethod
+    def backward(ctx, go):
         if torch.is_grad_enabled():  # create_graph: the gradient depends on go, which this call would hide
             raise _lib.SmelbError("balance_loss: there is no second derivative")
         mask, cu = ctx.saved_tensors if ctx.given else (None, None)
@@ -99,7 +94,7 @@ class _BalanceLossFn(torch.autograd.Function):
         d = torch.empty(T, E, dtype=torch.float32, device=dev)
         _lib.call_on(dev, "smelb_balance_loss_bwd", coef.data_ptr(), go.data_ptr(), _lib.ptr(mask), _lib.ptr(cu), S, T, E,
                      d.data_ptr(), _lib.stream_of(dev))
-        return d, None, None, None
+        return d, None
 
 
 def balance_loss(probs, topi, mask=None, cu_seqlens=None):
@@ -114,7 +109,20 @@ def balance_loss(probs, topi, mask=None, cu_seqlens=None):
 
     Differentiable w.r.t. probs, with the counts as constants; the same inputs give the same bits. Choices outside [0, E)
     are not counted and recorded in the status word (read_status)."""
-    return _BalanceLossFn.apply(probs, topi, mask, cu_seqlens)
+    p, ld, topi, mask = _tables("balance_loss", probs, topi, mask)
+    cu, shape = cu_seqlens, p.shape[1:]
+    if cu is not None:
+        if not cu.is_cuda or cu.device != p.device:
+            raise _lib.SmelbError(f"balance_loss: cu_seqlens on {cu.device}, probs on {p.device}")
+        if cu.dtype != torch.int32 or cu.dim() != 1 or cu.numel() < 2:
+            raise _lib.SmelbError(f"balance_loss: cu_seqlens must be int32 [sequences + 1] (got {cu.dtype} "
+                                  f"{tuple(cu.shape)})")
+        cu = cu.contiguous()
+        shape = (cu.numel() - 1, p.shape[1])
+    counts = torch.empty(shape, dtype=torch.int64, device=p.device)
+    tables = (p, ld, topi, mask, cu, counts)
+    loss = _BalanceLossFn.apply(probs, tables) if probs.requires_grad else _loss(*tables)[0]
+    return loss, counts
 
 
 def expert_usage(probs, topv, topi, mask=None):
