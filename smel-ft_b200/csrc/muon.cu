@@ -24,7 +24,8 @@ namespace smelb {
 namespace {
 
 constexpr int kThreads = 256, kWarps = 8;
-constexpr int kSplitCap = 128;  // columns of a chunk of the split way
+// Columns of a chunk of the split way: 16 to 66 KB.
+__host__ __device__ constexpr int split_cap(int nt) { return nt <= 4 ? 512 : 128; }
 constexpr int kDevErrWaitCluster = 16;  // a block waiting for its cluster's parts of the Gram matrix
 constexpr int kMaxSteps = 16, kMaxTensors = 48, kMaxD = 64;
 
@@ -260,16 +261,96 @@ __device__ __forceinline__ void load_vectors(const Args& a, const Tensor& t, con
   }
 }
 
-// Element q of columns [j0, j0 + w): its place in x and its offset in memory from (0, j0).
-__device__ __forceinline__ int element_at(const Tensor& t, int w, int q, int& i, int& j) {
+// Single elements of w columns, for matrices whose rows do not start on 16 bytes: calls f(u, offset in memory, place in x)
+// for up to U elements, u < U, between two calls of done(). A warp takes every eighth row of a wide matrix; a tall one is
+// contiguous, and a thread's next element is kThreads on.
+template <int U, class F, class G>
+__device__ __forceinline__ void elements(const Tensor& t, int w, int ld, F&& f, G&& done) {
   if (t.tall) {
-    j = q / t.d;
-    i = q - j * t.d;
-    return q;
+    int j = (int)__umulhi((uint32_t)threadIdx.x, t.by_d), i = threadIdx.x - j * t.d;
+    const int dj = (int)__umulhi((uint32_t)kThreads, t.by_d), di = kThreads - dj * t.d;
+    for (int q = threadIdx.x; q < w * t.d; q += U * kThreads) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (q + u * kThreads < w * t.d) f(u, q + u * kThreads, i * ld + j);
+        i += di;
+        j += dj;
+        if (i >= t.d) {
+          i -= t.d;
+          ++j;
+        }
+      }
+      done();
+    }
+  } else {
+    const int lane = threadIdx.x & 31;
+    for (int i = threadIdx.x >> 5; i < t.d; i += kWarps)
+      for (int j = lane; j < w; j += U * 32) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (j + u * 32 < w) f(u, i * t.L + j + u * 32, i * ld + j + u * 32);
+        done();
+      }
   }
-  i = q / w;
-  j = q - i * w;
-  return i * t.L + j;
+}
+
+template <typename T, bool MUON>
+__device__ __noinline__ void load_elements(const Args& a, const Tensor& t, const T* g, float* m, int w, float* x, int ld,
+                                           bool first) {
+  constexpr int U = 8;
+  float rg[U], rm[U];
+  int at[U], in[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) at[u] = -1;
+  elements<U>(t, w, ld,
+              [&](int u, int from, int to) {
+                at[u] = from;
+                in[u] = to;
+                rg[u] = to_f(g[from]);
+                if (MUON) rm[u] = m[from];
+              },
+              [&] {
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                  if (at[u] >= 0) {
+                    float v = rg[u];
+                    if (MUON) {
+                      v = update(a, v, rm[u], first);
+                      if (first) m[at[u]] = rm[u];
+                    }
+                    x[in[u]] = v;
+                    at[u] = -1;
+                  }
+              });
+}
+
+// The result o at a place whose present value is p.
+template <bool MUON>
+__device__ __forceinline__ float result(const Args& a, const Tensor& t, float o, float p) {
+  return MUON ? fmaf(-t.step, o, p * a.decay) : o;
+}
+
+template <typename T, bool MUON>
+__device__ __noinline__ void store_elements(const Args& a, const Tensor& t, T* p, int w, const float* x, int ld) {
+  constexpr int U = 8;
+  float rp[U];
+  int at[U], in[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) at[u] = -1;
+  elements<U>(t, w, ld,
+              [&](int u, int to, int from) {
+                at[u] = to;
+                in[u] = from;
+                if (MUON) rp[u] = to_f(p[to]);
+              },
+              [&] {
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                  if (at[u] >= 0) {
+                    put(p + at[u], result<MUON>(a, t, x[in[u]], MUON ? rp[u] : 0.f));
+                    at[u] = -1;
+                  }
+              });
 }
 
 // Columns [j0, j0 + w) (j0 a multiple of 8) into x, zeros up to the next multiple of 8 and in the rows that fill the
@@ -286,17 +367,7 @@ __device__ __forceinline__ void load_slice(const Args& a, const Tensor& t, long 
   } else if (vec) {
     load_vectors<T, MUON, false>(a, t, g, m, w, x, ld, first);
   } else {
-    for (int q = threadIdx.x; q < w * t.d; q += kThreads) {
-      int i, j;
-      const int at = element_at(t, w, q, i, j);
-      float v = to_f(g[at]);
-      if (MUON) {
-        float b = m[at];
-        v = update(a, v, b, first);
-        if (first) m[at] = b;
-      }
-      x[i * ld + j] = v;
-    }
+    load_elements<T, MUON>(a, t, g, m, w, x, ld, first);
   }
   const int w8 = (w + 7) & ~7;
   if (w < w8)
@@ -307,12 +378,6 @@ __device__ __forceinline__ void load_slice(const Args& a, const Tensor& t, long 
   if (t.d < NT * 8)
     for (int i = t.d; i < NT * 8; ++i)
       for (int j = threadIdx.x; j < w8; j += kThreads) x[i * ld + j] = 0.f;
-}
-
-// The result o at a place whose present value is p.
-template <bool MUON>
-__device__ __forceinline__ float result(const Args& a, const Tensor& t, float o, float p) {
-  return MUON ? fmaf(-t.step, o, p * a.decay) : o;
 }
 
 template <typename T, bool MUON, bool TALL>
@@ -355,11 +420,7 @@ __device__ __forceinline__ void store_slice(const Args& a, const Tensor& t, long
   } else if (vec) {
     store_vectors<T, MUON, false>(a, t, p, w, x, ld);
   } else {
-    for (int q = threadIdx.x; q < w * t.d; q += kThreads) {
-      int i, j;
-      T* at = p + element_at(t, w, q, i, j);
-      put(at, result<MUON>(a, t, x[i * ld + j], MUON ? to_f(*at) : 0.f));
-    }
+    store_elements<T, MUON>(a, t, p, w, x, ld);
   }
 }
 
@@ -1088,15 +1149,15 @@ int blocks_needed(int nt, int L) {
 }
 
 static_assert(sizeof(Args) <= 4096, "kernel parameters");
-static_assert(kSplitCap <= kThreads * 2 / 4, "apply_plain takes a chunk at once from 48 rows on");
+static_assert(split_cap(8) <= kThreads * 2 / 4, "apply_plain takes a chunk at once from 48 rows on");
 
 // Matrices of one round of the split way: their partial Gram matrices and P are the workspace (50 KB each at 64 rows).
 constexpr long long kSplitRound = 4096;
 
 // Blocks for one matrix of the split way: as many chunks to each as leave eight blocks for an SM, and at most two blocks on
 // every SM for one matrix (their partial Gram matrices are added by one block).
-int split_blocks(long long matrices, int L) {
-  const long long chunks = (L + kSplitCap - 1) / kSplitCap;
+int split_blocks(int nt, long long matrices, int L) {
+  const long long chunks = (L + split_cap(nt) - 1) / split_cap(nt);
   const long long per =
       std::max({1LL, chunks * std::min(matrices, kSplitRound) / (148 * 8), (chunks + 295) / 296});
   return (int)((chunks + per - 1) / per);
@@ -1132,8 +1193,8 @@ int run_resident(Args& a, long long matrices, int maxL, cudaStream_t st) {
 template <int NT, typename T, bool MUON>
 int run_split(Args& a, long long matrices, int maxL, double* ws, cudaStream_t st) {
   using D_ = Dims<NT>;
-  a.blocks = split_blocks(matrices, maxL);
-  set_cap(a, kSplitCap);
+  a.blocks = split_blocks(NT, matrices, maxL);
+  set_cap(a, split_cap(NT));
   const long long x = (long long)NT * 8 * pitch(a.cap) * 4;
   const int blocks = a.blocks;
   for (a.first = 0; a.first < matrices; a.first += kSplitRound) {
@@ -1217,7 +1278,7 @@ long long workspace(const smelb_muon_tensor* t, int64_t n) {
   for_launches(t, n, [&](int nt, bool held, const int64_t*, int, long long matrices, int maxL) {
     if (!held) {
       const long long part = nt * (nt + 1) / 2 * 64, form = nt * nt * 64 + 2;
-      most = std::max(most, std::min(matrices, kSplitRound) * (split_blocks(matrices, maxL) * part + form) * 8);
+      most = std::max(most, std::min(matrices, kSplitRound) * (split_blocks(nt, matrices, maxL) * part + form) * 8);
     }
     return 0;
   });

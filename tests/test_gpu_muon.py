@@ -73,7 +73,8 @@ def check(out, x, **k):
 
 SHAPES = [(1, 1), (1, 7), (7, 1), (3, 5), (8, 8), (8, 9), (16, 16), (16, 2048), (2048, 16), (512, 16), (24, 703), (703, 24),
           (33, 100), (100, 31), (48, 513), (64, 64), (64, 65), (64, 2048), (2051, 64), (57, 1000), (5, 20001), (20001, 3),
-          (16, 40000), (40000, 12), (64, 6003), (1, 30000)]
+          (16, 40000), (40000, 12), (64, 6003), (1, 30000), (8, 55296), (24, 15001), (15872, 20), (32, 12000), (10495, 30),
+          (16, 26112), (60001, 8)]
 
 
 @pytest.mark.parametrize("m,n", SHAPES)
