@@ -1058,11 +1058,16 @@ __global__ void __launch_bounds__(form_warps<NT>() * 32) form_kernel(const __gri
   extern __shared__ __align__(16) double sm[];
   double *G = sm, *work = G + D_::MAT;
   const double* part = a.gram + (long long)blockIdx.x * a.blocks * D_::PART;
-  for (int q = threadIdx.x; q < D_::PART; q += FT) {
-    double s = 0.0;
+  for (int q = threadIdx.x * 2; q < D_::PART; q += FT * 2) {
+    double2 s = make_double2(0.0, 0.0);
 #pragma unroll 8
-    for (int b = 0; b < a.blocks; ++b) s += part[(long long)b * D_::PART + q];
-    spread<NT>(G, q, s);
+    for (int b = 0; b < a.blocks; ++b) {
+      const double2 v = *reinterpret_cast<const double2*>(part + (long long)b * D_::PART + q);
+      s.x += v.x;
+      s.y += v.y;
+    }
+    spread<NT>(G, q, s.x);
+    spread<NT>(G, q + 1, s.y);
   }
   __syncthreads();
   double* P;
@@ -1134,17 +1139,17 @@ int launch(F* kern, const Args& a, long long blocks, int threads, long long smem
 }
 
 // Columns of a resident block at most: 47 KB for 16 rows (four blocks to an SM; 1024 columns in two ran 7% slower on 1548
-// matrices of 16 x 512 .. 2048), 104 KB for 32 (two blocks).
+// matrices of 16 x 512 .. 2048), 106 KB for 32 (two blocks in clusters of up to four).
 constexpr int kMaxBlocks = 8;
-constexpr int block_cols(int nt) { return nt <= 2 ? 512 : 352; }
+constexpr int kBlockCols = 512;
 
 // Whether matrices of this size are held by a cluster: up to 32 rows, and no more columns than eight blocks hold.
-bool resident(int nt, int L) { return nt <= 4 && L <= block_cols(nt) * kMaxBlocks; }
+bool resident(int nt, int L) { return nt <= 4 && L <= kBlockCols * kMaxBlocks; }
 
 // Blocks that a resident matrix needs.
-int blocks_needed(int nt, int L) {
+int blocks_needed(int L) {
   int c = 1;
-  while (L > block_cols(nt) * c) c *= 2;
+  while (L > kBlockCols * c) c *= 2;
   return c;
 }
 
@@ -1154,8 +1159,8 @@ static_assert(split_cap(8) <= kThreads * 2 / 4, "apply_plain takes a chunk at on
 // Matrices of one round of the split way: their partial Gram matrices and P are the workspace (50 KB each at 64 rows).
 constexpr long long kSplitRound = 4096;
 
-// Blocks for one matrix of the split way: as many chunks to each as leave eight blocks for an SM, and at most two blocks on
-// every SM for one matrix (their partial Gram matrices are added by one block).
+// Blocks for one matrix of the split way: as many chunks to each as leave eight blocks for an SM, and at most 296 for one
+// matrix (their partial Gram matrices are added by one block).
 int split_blocks(int nt, long long matrices, int L) {
   const long long chunks = (L + split_cap(nt) - 1) / split_cap(nt);
   const long long per =
@@ -1171,7 +1176,7 @@ int run_resident(Args& a, long long matrices, int maxL, cudaStream_t st) {
   // few matrices: more blocks for each, down to 256 columns, until two are on every SM, and the same for all. Many: each
   // as many as it needs, short ones side by side in a cluster (a short matrix spread over the blocks of a long one would
   // form P in each of them, and a launch of its own would leave SMs idle at its end).
-  int c = blocks_needed(NT, maxL);
+  int c = blocks_needed(maxL);
   const bool few = matrices * c <= 148 * 4;
   while (few && c < kMaxBlocks && maxL > 256 * c && matrices * c < 296) c *= 2;
   a.blocks = c;
@@ -1180,7 +1185,7 @@ int run_resident(Args& a, long long matrices, int maxL, cudaStream_t st) {
   int cap = 32;
   for (int k = 0; k < a.n; ++k) {
     Tensor& t = a.t[k];
-    t.shift = few ? a.shift : log2_of(blocks_needed(NT, t.L));
+    t.shift = few ? a.shift : log2_of(blocks_needed(t.L));
     t.start = clusters;
     clusters += (t.batch + (c >> t.shift) - 1) >> (a.shift - t.shift);
     cap = std::max(cap, (((t.L + (1 << t.shift) - 1) >> t.shift) + 31) / 32 * 32);

@@ -127,9 +127,9 @@ def test_workspace_sizes():
     from smelb import _lib
     lib = _lib.load()
     ws = lib.smelb_orthogonalize_workspace_bytes
-    assert ws(12, 16, 2048) == 0 and ws(12, 2048, 16) == 0 and ws(5, 32, 2816) == 0 and ws(0, 64, 2048) == 0
-    assert ws(5, 32, 2817) > 0 and ws(1, 16, 4097) > 0 and ws(1, 33, 40) > 0
-    assert ws(1000, 64, 2048) >= 1000 * (36 + 64) * 64 * 8 and ws(1, 64, 1 << 20) >= 256 * 36 * 64 * 8
+    assert ws(12, 16, 2048) == 0 and ws(12, 2048, 16) == 0 and ws(5, 32, 4096) == 0 and ws(0, 64, 2048) == 0
+    assert ws(5, 32, 4097) > 0 and ws(1, 16, 4097) > 0 and ws(1, 33, 40) > 0
+    assert ws(1000, 64, 2048) >= 1000 * (36 + 64) * 64 * 8 and ws(1, 64, 1 << 20) >= 32 * 36 * 64 * 8
     assert ws(1 << 20, 64, 64) == ws(4096, 64, 64)  # rounds of 4096 matrices
     assert ws(1, 65, 65) == -1 and ws(-1, 16, 16) == -1
     t = (_lib.MuonTensor * 2)()
