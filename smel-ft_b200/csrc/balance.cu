@@ -64,23 +64,126 @@ __device__ __forceinline__ void seq_range(const int* cu, int s, long long T, lon
 
 __device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 
-// Number of sequences that end at or before row t: the first one that can hold it. Called by the whole block.
-__device__ __forceinline__ int first_seq(const int* cu, int S, long long t) {
-  int s0 = 0;
+// The sequences that can hold rows t0 .. t1: those from the first that ends behind t0 to the first that ends behind t1
+// (counted by the whole block, in one pass over their ends).
+__device__ __forceinline__ void sequences_of(const int* cu, int S, long long t0, long long t1, int& s0, int& s1) {
+  s0 = s1 = 0;
   if (cu)
     for (int base = 0; base < S; base += blockDim.x) {
       const int s = base + threadIdx.x;
-      s0 += __syncthreads_count(s < S && cu[s + 1] <= t);
+      const long long end = s < S ? cu[s + 1] : t1 + 1;
+      s0 += __syncthreads_count(end <= t0);
+      s1 += __syncthreads_count(end <= t1);
     }
-  return s0;
 }
 
-template <int VEC, bool USAGE>
-__global__ void __launch_bounds__(kTileThreads, USAGE ? 4 : 3) balance_tile_kernel(const TileArgs a) {
+// The sequence that holds row t (-1: none), among s0 .. s1.
+__device__ __forceinline__ int sequence_of(const int* cu, int S, long long t, int s0, int s1) {
+  if (!cu) return 0;
+  while (s0 < s1) {
+    const int mid = (s0 + s1) >> 1;
+    if (cu[mid + 1] <= t) s0 = mid + 1;
+    else s1 = mid;
+  }
+  return s0 < S && cu[s0] <= t && t < cu[s0 + 1] ? s0 : -1;
+}
+
+// A tile's rows by runs of one sequence. A run of kWarpRows rows or more, or a tile's only one, is summed by the block;
+// shorter ones, of which a tile of short sequences has many, by a warp each (a run costs the block 1.5 us of barriers).
+constexpr int kWarpRows = 32;
+struct Runs {
+  int seq[kMaxTileRows];         // sequence of each row
+  int begin[kMaxTileRows + 1];   // first row of each run, then the number of rows
+  int in_warp[kMaxTileRows / 32];
+  int n;
+};
+__device__ __forceinline__ void find_runs(Runs& runs, const int* cu, int S, long long t0, int rows) {
+  const int tid = threadIdx.x, lane = tid & 31;
+  int s0, s1;
+  sequences_of(cu, S, t0, t0 + rows - 1, s0, s1);
+  if (s0 == s1 && s0 < S && cu[s0] <= t0) {  // as most tiles of long sequences: one run
+    if (tid == 0) {
+      runs.seq[0] = s0;
+      runs.begin[0] = 0;
+      runs.begin[1] = rows;
+      runs.n = 1;
+    }
+    __syncthreads();
+    return;
+  }
+  if (tid < rows) runs.seq[tid] = sequence_of(cu, S, t0 + tid, s0, s1);
+  __syncthreads();
+  const bool head = tid < rows && (tid == 0 || runs.seq[tid] != runs.seq[tid - 1]);
+  const unsigned heads = __ballot_sync(0xffffffffu, head);
+  if (lane == 0 && tid < kMaxTileRows) runs.in_warp[tid / 32] = __popc(heads);
+  __syncthreads();
+  if (tid < kMaxTileRows) {
+    int k = __popc(heads & ((1u << lane) - 1));
+    for (int w = 0; w < tid / 32; ++w) k += runs.in_warp[w];
+    if (head) runs.begin[k] = tid;
+    if (tid == kMaxTileRows - 1) {
+      runs.n = k + (head ? 1 : 0);
+      runs.begin[runs.n] = rows;
+    }
+  }
+  __syncthreads();
+}
+
+// One run by one warp: rows [ra, rb), less than kWarpRows of them. h: the warp's table of counts.
+template <int VEC>
+__device__ __forceinline__ void warp_run(const TileArgs& a, const uint8_t* ok, int* h, long long t0, int ra, int rb,
+                                         long long rec) {
+  const int lane = threadIdx.x & 31, E = a.E, K = a.K;
+  for (int e = lane; e < E; e += 32) h[e] = 0;
+  const bool mine = ra + lane < rb && ok[ra + lane];
+  const unsigned kept = __ballot_sync(0xffffffffu, mine);
+  for (int i = ra * K + lane; i < rb * K; i += 32)
+    if (ok[K == 1 ? i : (int)__umulhi((uint32_t)i, a.by_k)]) {
+      const long long v = a.topi[t0 * K + i];
+      if (v >= 0 && v < E) atomicAdd(&h[(int)v], 1);
+      else dev_fail(a.err, kDevErrBadIndex);
+    }
+  __syncwarp();
+  for (int col = lane * VEC; col < E; col += 32 * VEC) {
+    const float* p = a.probs + t0 * a.ld + col;
+    float acc[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
+#pragma unroll 4
+    for (int r = ra; r < rb; ++r) {
+      float v[VEC];
+      if constexpr (VEC == 4) {
+        const float4 f = __ldg(reinterpret_cast<const float4*>(p + r * a.ld));
+        v[0] = f.x;
+        v[1] = f.y;
+        v[2] = f.z;
+        v[3] = f.w;
+      } else {
+        v[0] = __ldg(p + r * a.ld);
+      }
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) acc[j] += (kept >> (r - ra)) & 1 ? v[j] : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) a.rec_mass[rec * E + col + j] = acc[j];
+  }
+  for (int e = lane; e < E; e += 32) a.rec_cnt[rec * E + e] = h[e];
+  if (lane == 0) a.rec_n[rec] = __popc(kept);
+  __syncwarp();
+}
+
+// KIND: the loss over one sequence, the loss over packed ones, or the usage statistics (one sequence). Blocks to an SM by
+// what their registers hold without spilling in the loops (packed: 74 us a pass of 131072 x 256 at two, 86 at three).
+enum TileKind { kOne, kPacked, kUsage };
+template <int VEC, int KIND>
+__global__ void __launch_bounds__(kTileThreads, KIND == kUsage ? 4 : KIND == kPacked ? 2 : 3)
+    balance_tile_kernel(const TileArgs a) {
+  constexpr bool USAGE = KIND == kUsage, PACKED = KIND == kPacked;
   __shared__ uint8_t ok[kMaxTileRows];
   __shared__ int cnt[kMaxE];
   __shared__ float red[kTileThreads * VEC];
-  extern __shared__ float hist[];  // usage: [kTileWarps][E]
+  __shared__ Runs runs;  // packed
+  extern __shared__ float hist[];  // [kTileWarps][E]: the warps' weights (usage), or counts (short sequences)
   const int tid = threadIdx.x, E = a.E, K = a.K;
   const long long t0 = (long long)blockIdx.x * a.rows;
   const int rows = (int)min((long long)a.rows, a.T - t0);
@@ -95,13 +198,20 @@ __global__ void __launch_bounds__(kTileThreads, USAGE ? 4 : 3) balance_tile_kern
   if (tid < rows) ok[tid] = a.mask ? a.mask[t0 + tid] != 0 : 1;
   const int ncol = (E + VEC - 1) / VEC, lanes = kTileThreads / ncol;
   const int lane = tid / ncol, col = (tid - lane * ncol) * VEC;
-  int s = first_seq(a.cu, a.S, t0);
-  for (; s < a.S; ++s) {
-    long long lo, hi;
-    seq_range(a.cu, s, a.T, lo, hi);
-    if (lo >= t0 + rows) break;
-    const int ra = (int)(max(lo, t0) - t0), rb = (int)(min(hi, t0 + rows) - t0);
-    if (ra >= rb) continue;
+  int n_runs = 1;
+  if constexpr (PACKED) {
+    find_runs(runs, a.cu, a.S, t0, rows);
+    n_runs = runs.n;
+    if (n_runs > 1)
+      for (int k = tid >> 5; k < n_runs; k += kTileWarps) {
+        const int ra = runs.begin[k], rb = runs.begin[k + 1], s = runs.seq[ra];
+        if (s >= 0 && rb - ra < kWarpRows)
+          warp_run<VEC>(a, ok, reinterpret_cast<int*>(hist) + (tid >> 5) * E, t0, ra, rb, (long long)blockIdx.x + s);
+      }
+  }
+  for (int k = 0; k < n_runs; ++k) {
+    const int ra = PACKED ? runs.begin[k] : 0, rb = PACKED ? runs.begin[k + 1] : rows, s = PACKED ? runs.seq[ra] : 0;
+    if (s < 0 || (n_runs > 1 && rb - ra < kWarpRows)) continue;
     for (int e = tid; e < E; e += kTileThreads) cnt[e] = 0;
     if (USAGE)
       for (int i = tid; i < kTileWarps * E; i += kTileThreads) hist[i] = 0.f;
@@ -201,9 +311,44 @@ struct FinArgs {
   int* ticket;
 };
 
+// The last block to finish adds the parts of the sequences (gridDim.y each) in their order.
+__device__ __forceinline__ void finish_loss(const FinArgs& a) {
+  constexpr int WARPS = kFinThreads / 32;
+  __shared__ double sums[WARPS];
+  __shared__ int somes[WARPS];
+  __threadfence();
+  const volatile double* parts = a.part;
+  const volatile int* seqs = a.seq_n;
+  double sum = 0.0;
+  int some = 0;
+  for (long long i = threadIdx.x; i < (long long)a.S * gridDim.y; i += kFinThreads) sum += parts[i];
+  for (int i = threadIdx.x; i < a.S; i += kFinThreads) some += seqs[i];
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    some += __shfl_xor_sync(0xffffffffu, some, o);
+  }
+  if (threadIdx.x % 32 == 0) {
+    sums[threadIdx.x / 32] = sum;
+    somes[threadIdx.x / 32] = some;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    sum = 0.0;
+    some = 0;
+    for (int l = 0; l < WARPS; ++l) {
+      sum += sums[l];
+      some += somes[l];
+    }
+    const double inv = 1.0 / max(some, 1);
+    *a.loss = (float)(sum * inv);
+    a.coef[(long long)a.S * a.E] = (float)inv;
+  }
+}
+
 template <bool USAGE, int COLS>
 __global__ void __launch_bounds__(kFinThreads) balance_finish_kernel(const FinArgs a) {
-  constexpr int LANES = kFinThreads / COLS, WARPS = kFinThreads / 32;
+  constexpr int LANES = kFinThreads / COLS;
   __shared__ double sm[LANES][COLS + 1];
   __shared__ double sw[USAGE ? LANES : 1][COLS + 1];
   __shared__ int sc[LANES][COLS + 1];
@@ -276,37 +421,50 @@ __global__ void __launch_bounds__(kFinThreads) balance_finish_kernel(const FinAr
   }
   if (USAGE) return;
   __syncthreads();
-  if (!last) return;
-  // the last block to finish adds the blocks' parts in their order
-  __threadfence();
-  const volatile double* parts = a.part;
-  const volatile int* seqs = a.seq_n;
-  double sum = 0.0;
-  int some = 0;
-  for (long long i = threadIdx.x; i < (long long)gridDim.x * gridDim.y; i += kFinThreads) sum += parts[i];
-  for (int i = threadIdx.x; i < a.S; i += kFinThreads) some += seqs[i];
+  if (last) finish_loss(a);
+}
+
+// The same with a warp for 32 experts of a sequence, where sequences are short: at most a few records each.
+__global__ void __launch_bounds__(kFinThreads) balance_finish_short_kernel(const FinArgs a) {
+  __shared__ bool last;
+  const int s = blockIdx.x * (kFinThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31, E = a.E;
+  const int e = blockIdx.y * 32 + lane;
+  if (s < a.S) {
+    long long lo, hi;
+    seq_range(a.cu, s, a.T, lo, hi);
+    double m = 0.0;
+    long long c = 0, n = 0;
+    if (lo < hi) {
+      const int b1 = (int)((hi - 1) / a.rows);
+#pragma unroll 8
+      for (int b = (int)(lo / a.rows); b <= b1; ++b) {
+        const long long rec = (long long)b + s;
+        n += a.rec_n[rec];
+        if (e < E) {
+          m += a.rec_mass[rec * E + e];
+          c += a.rec_cnt[rec * E + e];
+        }
+      }
+    }
+    double part = 0.0;
+    if (e < E) {
+      const double f = n ? (double)E * (double)c / ((double)a.K * (double)n * (double)n) : 0.0;
+      a.counts[(long long)s * E + e] = c;
+      a.coef[(long long)s * E + e] = (float)f;
+      part = f * m;
+    }
 #pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    some += __shfl_xor_sync(0xffffffffu, some, o);
-  }
-  double* ws = &sm[0][0];
-  if (threadIdx.x % 32 == 0) {
-    ws[threadIdx.x / 32] = sum;
-    sn[threadIdx.x / 32] = some;
+    for (int o = 16; o; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+    if (lane == 0) {
+      a.part[(long long)s * gridDim.y + blockIdx.y] = part;
+      if (blockIdx.y == 0) a.seq_n[s] = n > 0;
+      __threadfence();
+    }
   }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    sum = 0.0;
-    some = 0;
-    for (int l = 0; l < WARPS; ++l) {
-      sum += ws[l];
-      some += sn[l];
-    }
-    const double inv = 1.0 / max(some, 1);
-    *a.loss = (float)(sum * inv);
-    a.coef[(long long)a.S * E] = (float)inv;
-  }
+  if (threadIdx.x == 0) last = atomicAdd(a.ticket, 1) == (int)(gridDim.x * gridDim.y) - 1;
+  __syncthreads();
+  if (last) finish_loss(a);
 }
 
 // dprobs[t, :] = go / S' * coef[s(t), :] on the kept rows of the sequences, 0 elsewhere.
@@ -319,15 +477,11 @@ __global__ void __launch_bounds__(kTileThreads)
   const long long t0 = (long long)blockIdx.x * rows_per;
   const int rows = (int)min((long long)rows_per, T - t0);
   const float g = *go * coef[(long long)S * E];
-  const int s0 = first_seq(cu, S, t0);
+  int s0, s1;
+  sequences_of(cu, S, t0, t0 + rows - 1, s0, s1);
   if (tid < rows) {
     const long long t = t0 + tid;
-    int s = s0;
-    if (cu) {
-      while (s < S && cu[s + 1] <= t) ++s;
-      if (s < S && cu[s] > t) s = S;
-    }
-    seq[tid] = s < S && (!mask || mask[t]) ? s : -1;
+    seq[tid] = !mask || mask[t] ? sequence_of(cu, S, t, s0, s1) : -1;
   }
   __syncthreads();
   const int ncol = (E + VEC - 1) / VEC, lanes = kTileThreads / ncol;
@@ -360,15 +514,15 @@ int tile_rows(long long T) {
 struct Layout {
   long long mass, weight, cnt, n, part, seq_n, ticket, total;
   int rows, tiles;
-  int cols;  // experts of a finishing block
+  int cols;  // experts of a finishing block (0: a warp for 32 experts of a sequence)
 };
 
 Layout layout(long long T, long long E, long long S, bool usage) {
   Layout l{};
   l.rows = tile_rows(T);
   l.tiles = (int)((T + l.rows - 1) / l.rows);
-  l.cols = S * E < 32 * 148 ? 8 : 32;
-  const long long recs = l.tiles + S, eb = (E + l.cols - 1) / l.cols;
+  l.cols = S > 16 && l.tiles < 4 * S ? 0 : S * E < 32 * 148 ? 8 : 32;
+  const long long recs = l.tiles + S, eb = (E + 31) / 32 * (l.cols == 8 ? 4 : 1);
   long long o = 0;
   auto take = [&](long long bytes) {
     const long long at = o;
@@ -400,9 +554,11 @@ template <bool USAGE>
 int run_tiles(const TileArgs& t, int tiles, cudaStream_t st) {
   if (!tiles) return kOk;
   const bool vec = t.E % 4 == 0 && t.ld % 4 == 0 && ((uintptr_t)t.probs & 15) == 0;
-  const size_t smem = USAGE ? (size_t)kTileWarps * t.E * sizeof(float) : 0;
-  if (vec) balance_tile_kernel<4, USAGE><<<tiles, kTileThreads, smem, st>>>(t);
-  else balance_tile_kernel<1, USAGE><<<tiles, kTileThreads, smem, st>>>(t);
+  const size_t smem = USAGE || t.cu ? (size_t)kTileWarps * t.E * sizeof(float) : 0;
+  constexpr int kAlone = USAGE ? kUsage : kOne, kSeqs = USAGE ? kUsage : kPacked;
+  auto kern = t.cu ? (vec ? balance_tile_kernel<4, kSeqs> : balance_tile_kernel<1, kSeqs>)
+                   : (vec ? balance_tile_kernel<4, kAlone> : balance_tile_kernel<1, kAlone>);
+  kern<<<tiles, kTileThreads, smem, st>>>(t);
   SMELB_CUDA(cudaGetLastError());
   count_launch();
   return kOk;
@@ -410,8 +566,12 @@ int run_tiles(const TileArgs& t, int tiles, cudaStream_t st) {
 
 template <bool USAGE>
 int run_finish(const FinArgs& f, int cols, cudaStream_t st) {
-  const dim3 grid((unsigned)f.S, (unsigned)((f.E + cols - 1) / cols));
-  if (cols == 8) balance_finish_kernel<USAGE, 8><<<grid, kFinThreads, 0, st>>>(f);
+  const dim3 grid((unsigned)f.S, (unsigned)((f.E + std::max(cols, 1) - 1) / std::max(cols, 1)));
+  if (cols == 0) {
+    const int per = kFinThreads / 32;
+    balance_finish_short_kernel<<<dim3((unsigned)((f.S + per - 1) / per), (unsigned)((f.E + 31) / 32)), kFinThreads, 0,
+                                  st>>>(f);
+  } else if (cols == 8) balance_finish_kernel<USAGE, 8><<<grid, kFinThreads, 0, st>>>(f);
   else balance_finish_kernel<USAGE, 32><<<grid, kFinThreads, 0, st>>>(f);
   SMELB_CUDA(cudaGetLastError());
   count_launch();

@@ -83,6 +83,10 @@ def test_balance_loss_one_sequence(dev, T, E, K, masked):
     (700, 128, 8, [5, 30, 31, 500, 650]),              # rows before the first and behind the last sequence
     (40000, 256, 8, [0, 1, 39000, 39100, 39998]),      # one long sequence over many tiles
     (33, 7, 2, list(range(34))),                       # every row a sequence
+    (3000, 512, 8, sorted((i * 37) % 2990 for i in range(400))),   # a few rows each
+    (6000, 33, 3, [7] + list(range(10, 5000, 31)) + [5990]),        # runs just below a warp's, then a long one
+    (5000, 128, 8, list(range(0, 5000, 33)) + [5000]),              # and just above
+    (24, 60, 1, sorted((i * 7) % 25 for i in range(258))),          # more sequences than rows
     (2000, 64, 8, [0] * 700 + [1000] * 900 + [2000]),  # more sequences than a block has threads, most empty
 ])
 @pytest.mark.parametrize("masked", [False, True])
