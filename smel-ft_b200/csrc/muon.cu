@@ -7,8 +7,10 @@
 //   S = a I + b G + c G^2;   P <- S P;   G <- S G S.
 // Precision. The steps grow a singular value near zero by a^steps (485 for the usual polynomial), and an error delta in
 // G moves the result by delta / sigma^2, so gradients of low rank (few tokens reached the expert) come out up to 3e-4
-// off when G is held in fp32. G and the d x d matrices are fp64, on the fp64 matrix instruction (m8n8k4); the product
-// with x is fp32 where P is small and fp64 elsewhere.
+// off when G is held in fp32, and 6e-5 with the last product alone in fp32 (P has entries up to 485 there, and the sums
+// cancel them). All of it is fp64, on the fp64 matrix instruction (m8n8k4), and rounded once. An fp32 last product for
+// the updates that allow it was built and was no faster (192 x 64 x 2048: 287 us against 278, 512 x 16 x 2048: 69 against 66).
+// The momentum update itself is rounded to fp32, as its buffer is.
 //
 // Two ways, by the size of a matrix:
 //   resident  a cluster of 1 to 8 blocks holds one matrix in shared memory and reads it once (ortho_kernel)
@@ -24,7 +26,7 @@ namespace smelb {
 namespace {
 
 constexpr int kThreads = 256, kWarps = 8;
-// Columns of a chunk of the split way: 16 to 66 KB.
+// Columns of a chunk of the split way: 16 to 66 KB (512 columns up to 32 rows: 169 us for 300 x 16 x 8192, 335 with 128).
 __host__ __device__ constexpr int split_cap(int nt) { return nt <= 4 ? 512 : 128; }
 constexpr int kDevErrWaitCluster = 16;  // a block waiting for its cluster's parts of the Gram matrix
 constexpr int kMaxSteps = 16, kMaxTensors = 48, kMaxD = 64;
@@ -59,7 +61,7 @@ struct Args {
   double eps;
   int* err;      // status words
   double* gram;  // split: [matrix][block][PART] partial Gram matrices
-  double* form;  // split: [matrix][NT * NT * 64 + 2] P and whether it is plain
+  double* form;  // split: [matrix][NT * NT * 64] P
   double coef[kMaxSteps][3];
 };
 
@@ -713,13 +715,10 @@ __device__ __forceinline__ void iterate_small(const Args& a, double* G, double* 
   }
 }
 
-// From the Gram matrix G of x (unscaled) to P with P x = the polynomial of x, in M[0] or M[1] (returned through P). work
-// holds S, V, M[0], M[1]. Returns whether no entry of P / inv (the polynomial's own matrix) is above kMaxPlain: the
-// product with x may then be fp32, whose d roundings stay near 2^-22 of the result. Gradients of low rank have entries
-// up to 485, and the sum cancels them.
-constexpr double kMaxPlain = 8.0;
+// From the Gram matrix G of x (unscaled) to P with P x = the polynomial of x, in M[0] or M[1] (returned). work holds S (two
+// up to 16 rows), V, M[0], M[1].
 template <int NT, int WARPS>
-__device__ bool iterate(const Args& a, double* G, double* work, double*& P) {
+__device__ double* iterate(const Args& a, double* G, double* work) {
   using D_ = Dims<NT>;
   double *S = work, *V = work + D_::MAT, *M = work + 2 * D_::MAT;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -819,23 +818,10 @@ __device__ bool iterate(const Args& a, double* G, double* work, double*& P) {
     }
   }
   __syncthreads();
-  P = M + ((a.steps - 1) & 1) * D_::MAT;
-  // the scale itself has to be a normal fp32 number with room for the sums
-  bool plain = inv > 1e-30 && inv < 1e30;
-  for (int q = threadIdx.x; q < D_::MAT; q += WARPS * 32) {
-    plain = plain && fabs(P[q]) <= kMaxPlain;  // false for NaN
-    P[q] *= inv;
-  }
-  return __syncthreads_and(plain);
-}
-
-// P's fp32 copy, row k then column i.
-template <int NT>
-__device__ __forceinline__ void round_form(const double* P, float* Pf) {
-  for (int q = threadIdx.x; q < Dims<NT>::MAT; q += kThreads) {
-    const int tile = q >> 6, i = (tile / NT) * 8 + ((q >> 3) & 7), k = (tile % NT) * 8 + (q & 7);
-    Pf[k * NT * 8 + i] = (float)P[q];
-  }
+  double* P = M + ((a.steps - 1) & 1) * D_::MAT;
+  for (int q = threadIdx.x; q < D_::MAT; q += WARPS * 32) P[q] *= inv;
+  __syncthreads();
+  return P;
 }
 
 // x <- P x in place in fp64: a warp owns C groups of eight columns at a time. Up to 16 rows P stays in registers.
@@ -886,43 +872,6 @@ __device__ __forceinline__ void apply(const double* P, float* x, int ld, int w) 
           *reinterpret_cast<float2*>(x + (8 * i + r) * ld + j + g * kWarps * 8 + 2 * c) =
               make_float2((float)o[g][i][0], (float)o[g][i][1]);
       }
-  }
-}
-
-// The same in fp32: a thread owns two columns and D / RG rows of the result, and reads row k of P as a broadcast. From 48
-// rows on (RG = 4) the four warps of a column write when all have read; w is at most kThreads * 2 / RG there.
-template <int NT>
-__device__ __forceinline__ void apply_plain(const float* Pf, float* x, int ld, int w) {
-  constexpr int D = NT * 8, RG = NT >= 6 ? 4 : 1, R = D / RG;
-  const int r0 = RG == 1 ? 0 : threadIdx.x / (kThreads / RG) * R;
-  for (int j = (threadIdx.x % (kThreads / RG)) * 2; j < w || RG > 1; j += kThreads * 2 / RG) {
-    float o[R][2];
-#pragma unroll
-    for (int i = 0; i < R; ++i) o[i][0] = o[i][1] = 0.f;
-    if (j < w) {
-#pragma unroll 4
-      for (int k = 0; k < D; ++k) {
-        const float2 v = *reinterpret_cast<const float2*>(x + k * ld + j);
-#pragma unroll
-        for (int i = 0; i < R; i += 4) {
-          const float4 p = *reinterpret_cast<const float4*>(Pf + k * D + r0 + i);
-          o[i][0] = fmaf(p.x, v.x, o[i][0]);
-          o[i][1] = fmaf(p.x, v.y, o[i][1]);
-          o[i + 1][0] = fmaf(p.y, v.x, o[i + 1][0]);
-          o[i + 1][1] = fmaf(p.y, v.y, o[i + 1][1]);
-          o[i + 2][0] = fmaf(p.z, v.x, o[i + 2][0]);
-          o[i + 2][1] = fmaf(p.z, v.y, o[i + 2][1]);
-          o[i + 3][0] = fmaf(p.w, v.x, o[i + 3][0]);
-          o[i + 3][1] = fmaf(p.w, v.y, o[i + 3][1]);
-        }
-      }
-    }
-    if (RG > 1) __syncthreads();
-    if (j < w) {
-#pragma unroll
-      for (int i = 0; i < R; ++i) *reinterpret_cast<float2*>(x + (r0 + i) * ld + j) = make_float2(o[i][0], o[i][1]);
-    }
-    if (RG > 1) break;
   }
 }
 
@@ -1001,15 +950,8 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 ? 4 : 2) ortho_kernel(const 
   }
   if (a.blocks > 1) cluster_arrive_relaxed();  // for the exit: this block's pushes are under way
   __syncthreads();
-  double* P;
-  if (iterate<NT, kWarps>(a, G, work, P)) {
-    float* Pf = reinterpret_cast<float*>(G);
-    round_form<NT>(P, Pf);
-    __syncthreads();
-    apply_plain<NT>(Pf, x, ld, w);
-  } else {
-    apply<NT>(P, x, ld, w);
-  }
+  const double* P = iterate<NT, kWarps>(a, G, work);
+  apply<NT>(P, x, ld, w);
   __syncthreads();
   if (w) store_slice<T, MUON>(a, t, base, j0, w, x, ld);
   if (a.blocks > 1) cluster_wait();
@@ -1070,14 +1012,12 @@ __global__ void __launch_bounds__(form_warps<NT>() * 32) form_kernel(const __gri
     spread<NT>(G, q + 1, s.y);
   }
   __syncthreads();
-  double* P;
-  const bool plain = iterate<NT, form_warps<NT>()>(a, G, work, P);
-  double* out = a.form + (long long)blockIdx.x * (D_::MAT + 2);
+  const double* P = iterate<NT, form_warps<NT>()>(a, G, work);
+  double* out = a.form + (long long)blockIdx.x * D_::MAT;
   for (int q = threadIdx.x; q < D_::MAT; q += FT) out[q] = P[q];
-  if (threadIdx.x == 0) out[D_::MAT] = plain ? 1.0 : 0.0;
 }
 
-// Split: x <- P x, read and written once more. Bound by the fp64 units where P is large (192 x 64 x 2048: 133 us, 87 at their
+// Split: x <- P x, read and written once more. Bound by the fp64 units (192 x 64 x 2048: 133 us, 87 at their
 // rate); as many blocks to an SM as the registers of the load allow.
 template <int NT, typename T, bool MUON>
 __global__ void __launch_bounds__(kThreads, NT >= 6 && !MUON && sizeof(T) == 4 ? 3 : 2)
@@ -1089,17 +1029,13 @@ __global__ void __launch_bounds__(kThreads, NT >= 6 && !MUON && sizeof(T) == 4 ?
   const long long mat = blockIdx.x / a.blocks;
   const Tensor& t = tensor_of(a, a.first + mat);
   const long long base = (a.first + mat - t.start) * t.d * t.L;
-  const double* form = a.form + mat * (D_::MAT + 2);
-  const bool plain = form[D_::MAT] != 0.0;
-  if (plain) round_form<NT>(form, reinterpret_cast<float*>(sm));
-  else
-    for (int q = threadIdx.x; q < D_::MAT; q += kThreads) sm[q] = form[q];
+  const double* form = a.form + mat * D_::MAT;
+  for (int q = threadIdx.x; q < D_::MAT; q += kThreads) sm[q] = form[q];
   for (int j0 = block * a.cap; j0 < t.L; j0 += a.blocks * a.cap) {
     const int w = min(a.cap, t.L - j0);
     load_slice<NT, T, MUON>(a, t, base, j0, w, x, ld, false);
     __syncthreads();
-    if (plain) apply_plain<NT>(reinterpret_cast<float*>(sm), x, ld, w);
-    else apply<NT>(sm, x, ld, w);
+    apply<NT>(sm, x, ld, w);
     __syncthreads();
     store_slice<T, MUON>(a, t, base, j0, w, x, ld);
     __syncthreads();
@@ -1143,7 +1079,8 @@ int launch(F* kern, const Args& a, long long blocks, int threads, long long smem
 constexpr int kMaxBlocks = 8;
 constexpr int kBlockCols = 512;
 
-// Whether matrices of this size are held by a cluster: up to 32 rows, and no more columns than eight blocks hold.
+// Whether matrices of this size are held by a cluster: up to 32 rows, and no more columns than eight blocks hold (1548
+// matrices of rank 16 the split way: 236 us a step against 144; 512 x 16 x 2048: 85 against 69).
 bool resident(int nt, int L) { return nt <= 4 && L <= kBlockCols * kMaxBlocks; }
 
 // Blocks that a resident matrix needs.
@@ -1154,7 +1091,6 @@ int blocks_needed(int L) {
 }
 
 static_assert(sizeof(Args) <= 4096, "kernel parameters");
-static_assert(split_cap(8) <= kThreads * 2 / 4, "apply_plain takes a chunk at once from 48 rows on");
 
 // Matrices of one round of the split way: their partial Gram matrices and P are the workspace (50 KB each at 64 rows).
 constexpr long long kSplitRound = 4096;
@@ -1175,7 +1111,8 @@ int run_resident(Args& a, long long matrices, int maxL, cudaStream_t st) {
   using D_ = Dims<NT>;
   // few matrices: more blocks for each, down to 256 columns, until two are on every SM, and the same for all. Many: each
   // as many as it needs, short ones side by side in a cluster (a short matrix spread over the blocks of a long one would
-  // form P in each of them, and a launch of its own would leave SMs idle at its end).
+  // form P in each of them, and a launch of its own would leave SMs idle at its end: 1548 matrices in 191, 154 and, as
+  // here, 142 us).
   int c = blocks_needed(maxL);
   const bool few = matrices * c <= 148 * 4;
   while (few && c < kMaxBlocks && maxL > 256 * c && matrices * c < 296) c *= 2;
@@ -1282,7 +1219,7 @@ long long workspace(const smelb_muon_tensor* t, int64_t n) {
   long long most = 0;
   for_launches(t, n, [&](int nt, bool held, const int64_t*, int, long long matrices, int maxL) {
     if (!held) {
-      const long long part = nt * (nt + 1) / 2 * 64, form = nt * nt * 64 + 2;
+      const long long part = nt * (nt + 1) / 2 * 64, form = nt * nt * 64;
       most = std::max(most, std::min(matrices, kSplitRound) * (split_blocks(nt, matrices, maxL) * part + form) * 8);
     }
     return 0;
