@@ -9,7 +9,7 @@
 // G moves the result by delta / sigma^2, so gradients of low rank (few tokens reached the expert) come out up to 3e-4
 // off when G is held in fp32, and 6e-5 with the last product alone in fp32 (P has entries up to 485 there, and the sums
 // cancel them). All of it is fp64, on the fp64 matrix instruction (m8n8k4), and rounded once. An fp32 last product for
-// the updates that allow it was built and was no faster (192 x 64 x 2048: 287 us against 278, 512 x 16 x 2048: 69 against 66).
+// the updates that allow it was built and was no faster (192 x 64 x 2048: 287 us against 278; 512 x 16 x 2048: 69, 66).
 // The momentum update itself is rounded to fp32, as its buffer is.
 //
 // Two ways, by the size of a matrix:
@@ -764,8 +764,10 @@ __device__ double* iterate(const Args& a, double* G, double* work) {
         __syncthreads();
         if (part < PARTS) {
           load_row<NT>(S, line, row);
-          if (!last) strip<NT, PARTS>(row, G, line, part, [&](const Spot<NT>& t, double (&c)[2]) { put_tile<NT>(V, t, c); });
-          if (step) strip<NT, PARTS>(row, from, line, part, [&](const Spot<NT>& t, double (&c)[2]) { put_tile<NT>(to, t, c); });
+          if (!last)
+            strip<NT, PARTS>(row, G, line, part, [&](const Spot<NT>& t, double (&c)[2]) { put_tile<NT>(V, t, c); });
+          if (step)
+            strip<NT, PARTS>(row, from, line, part, [&](const Spot<NT>& t, double (&c)[2]) { put_tile<NT>(to, t, c); });
         }
         if (last) break;
         __syncthreads();
@@ -886,12 +888,12 @@ __device__ __forceinline__ const Tensor& tensor_of(const Args& a, long long at) 
   return a.t[ti];
 }
 
-// Resident: the blocks of a cluster hold one matrix, or a few short ones, `cap` columns each at most. Their parts of the Gram matrix go to every
-// block's shared memory by asynchronous stores that the receiver's barrier counts: one way, and without the fence over
-// the stores to the momentum buffer that a cluster barrier would need.
-// Bound: one matrix at a time by latency (7.0 us for 12 matrices of 16 x 2048: of 13000 cycles 4100 the polynomial, 1650 the
-// last product, 1150 the loads); many by HBM and the fp64 units together (a Muon step of 1548 matrices of rank 16, 634 MB:
-// 142 us, 4.5 TB/s, the units half busy; loads and stores alone take 106).
+// Resident: the blocks of a cluster hold one matrix, or a few short ones, `cap` columns each at most. Their parts of the
+// Gram matrix go to every block of the matrix by asynchronous stores into its shared memory that the receiver's barrier
+// counts: one way, and without the fence over the stores to the momentum buffer that a cluster barrier would need.
+// Bound: one matrix at a time by latency (7.0 us for 12 matrices of 16 x 2048: of 13000 cycles 4100 the polynomial, 1650
+// the last product, 1150 the loads); many by HBM and the fp64 units together (a Muon step of 1548 matrices of rank 16,
+// 634 MB: 142 us, 4.5 TB/s, the units half busy; loads and stores alone take 106).
 template <int NT, typename T, bool MUON>
 __global__ void __launch_bounds__(kThreads, NT <= 2 ? 4 : 2) ortho_kernel(const __grid_constant__ Args a) {
   using D_ = Dims<NT>;
@@ -957,8 +959,9 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 ? 4 : 2) ortho_kernel(const 
   if (a.blocks > 1) cluster_wait();
 }
 
-// Split: block b of a matrix takes the chunks b, b + blocks, ... of `cap` columns. Bound by the fp64 units: 192 x 64 x 2048 in
-// 87 us, 49 at their rate; three blocks to an SM, as two (94 us) leave them idle while a block loads.
+// Split: block b of a matrix takes the chunks b, b + blocks, ... of `cap` columns. Bound by the fp64 units: 192 x 64 x 2048
+// in 82 us, 49 at their rate; three blocks to an SM where the registers allow it, as two (94 us) leave the units idle
+// while a block loads.
 template <int NT, typename T, bool MUON>
 __global__ void __launch_bounds__(kThreads, NT == 6 || MUON || sizeof(T) == 2 ? 2 : 3)
     gram_kernel(const __grid_constant__ Args a) {
