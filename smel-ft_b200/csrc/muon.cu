@@ -728,6 +728,7 @@ __device__ double* iterate(const Args& a, double* G, double* work) {
   for (int o = NT == 1 ? 4 : NT == 2 ? 8 : 16; o; o >>= 1) tr += __shfl_xor_sync(0xffffffffu, tr, o);
   const double inv = 1.0 / (sqrt(tr) + a.eps);
   if constexpr (2 * NT * NT <= WARPS) {
+    __syncthreads();  // every warp has its trace: the chain overwrites G without waiting for the others
     iterate_small<NT>(a, G, work, inv);
     M = work + 3 * D_::MAT;
   } else {
