@@ -135,6 +135,7 @@ __device__ __forceinline__ void warp_run(const TileArgs& a, const uint8_t* ok, i
                                          long long rec) {
   const int lane = threadIdx.x & 31, E = a.E, K = a.K;
   for (int e = lane; e < E; e += 32) h[e] = 0;
+  __syncwarp();  // the lanes add to each other's entries, and a vote orders no memory
   const bool mine = ra + lane < rb && ok[ra + lane];
   const unsigned kept = __ballot_sync(0xffffffffu, mine);
   for (int i = ra * K + lane; i < rb * K; i += 32)
