@@ -934,11 +934,12 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 ? 4 : 2) ortho_kernel(const 
   __syncthreads();
   gram<NT, 0>(x, ld, w, threadIdx.x >> 5, acc);
   if (a.blocks > 1) cluster_wait();  // every block's barrier is set up
+  bool there = true;
   if (blocks > 1) {
     reduce_warps<NT>(acc, work, [&](int q, double v0, double v1) {
       for (int r = 0; r < blocks; ++r) push(slots + rank * D_::PART + q, &bar, first + r, v0, v1);
     });
-    mbar_wait(&bar, 0, a.err, kDevErrWaitCluster, blockIdx.x);
+    there = mbar_wait(&bar, 0, a.err, kDevErrWaitCluster, blockIdx.x);
     for (int q = threadIdx.x; q < D_::PART; q += kThreads) {
       double s = 0.0;
 #pragma unroll 4
@@ -952,7 +953,13 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 ? 4 : 2) ortho_kernel(const 
     });
   }
   if (a.blocks > 1) cluster_arrive_relaxed();  // for the exit: this block's pushes are under way
-  __syncthreads();
+  // A part that did not come in time is recorded, and this block leaves its columns of the parameter or the output as they
+  // were. The others' pushes may still be on their way into its shared memory: it stays until they have landed.
+  if (!__syncthreads_and(there)) {
+    cluster_wait();
+    mbar_wait(&bar, 0, a.err, kDevErrWaitCluster, blockIdx.x);
+    return;
+  }
   const double* P = iterate<NT, kWarps>(a, G, work);
   apply<NT>(P, x, ld, w);
   __syncthreads();

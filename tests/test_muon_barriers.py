@@ -110,3 +110,68 @@ def test_the_kernel_has_the_barrier():
     body = text[text.index("__device__ double* iterate("):]
     trace = body[body.index("tr +="):body.index("iterate_small<NT>(")]
     assert re.search(r"__shfl_xor_sync.*__syncthreads\(\);", trace, re.S)
+
+
+def cluster(blocks, seed, give_up=True):
+    """The exchange of the Gram parts (ortho_kernel) with pushes that take any time and waits that may give up: per block
+    whether it stored, and what landed in a block that had left."""
+    rng = random.Random(seed)
+    landed, left, stored, lost = [0] * blocks, [False] * blocks, [False] * blocks, []
+    arrivals = {"up": 0, "exit": 0}
+    flying = []  # receivers of pushes under way
+
+    def block(r):
+        arrivals["up"] += 1
+        yield lambda: arrivals["up"] == blocks
+        flying.extend(range(blocks))
+        there = True
+        if give_up and rng.random() < 0.3:
+            there = landed[r] == blocks  # the wait's limit, whatever has come by now
+        else:
+            yield lambda: landed[r] == blocks
+        arrivals["exit"] += 1
+        if there:
+            stored[r] = landed[r] == blocks
+            assert stored[r]
+        yield lambda: arrivals["exit"] == blocks
+        if not there:
+            yield lambda: landed[r] == blocks
+        left[r] = True
+
+    runs = {r: block(r) for r in range(blocks)}
+    until = {r: lambda: True for r in range(blocks)}
+    while runs or flying:
+        can = [r for r in runs if until[r]()]
+        assert can or flying
+        if flying and (not can or rng.random() < 0.2):
+            to = flying.pop(rng.randrange(len(flying)))
+            landed[to] += 1
+            lost += [to] if left[to] else []
+        else:
+            r = rng.choice(can)
+            until[r] = next(runs[r], None)
+            if until[r] is None:
+                del runs[r]
+    return stored, lost
+
+
+@pytest.mark.parametrize("blocks", [2, 4, 8])
+def test_pushes_land_in_blocks_that_are_still_there(blocks):
+    """A block whose wait gives up stores nothing and stays until the others' parts have landed; the rest is not disturbed."""
+    some = 0
+    for seed in range(400):
+        stored, lost = cluster(blocks, seed)
+        assert lost == []
+        some += not all(stored)
+        assert cluster(blocks, seed, give_up=False) == ([True] * blocks, [])
+    assert some
+
+
+def test_the_kernel_heeds_the_wait():
+    with open(SOURCE) as f:
+        text = f.read()
+    body = text[text.index(" ortho_kernel(const"):]
+    body = body[:body.index("\n}\n")]
+    waits = re.findall(r"(\w+ = )?mbar_wait\(", body)
+    assert len(waits) == 2 and waits[0]
+    assert body.index("__syncthreads_and(") < body.index("iterate<") < body.index("store_slice<")
