@@ -17,6 +17,8 @@
 //   split     many blocks add partial Gram matrices of one matrix, one block forms P, many blocks apply it
 //             (gram_kernel, form_kernel, product_kernel); x is read twice
 #include <algorithm>
+#include <atomic>
+#include <mutex>
 
 #include "common.cuh"
 #include "host.h"
@@ -1066,10 +1068,28 @@ void set_cap(Args& a, int cap) {
   }
 }
 
-template <typename F>
-int launch(F* kern, const Args& a, long long blocks, int threads, long long smem, int cluster, cudaStream_t st) {
+// Raises the kernel's limit of shared memory on this device, never lowers it: another thread may be about to launch it with
+// the size that it has asked for.
+template <auto KERN>
+int raise_smem(long long bytes) {
+  static std::mutex mu;
+  static std::atomic<long long> raised[64];
+  int dev = 0;
+  SMELB_CUDA(cudaGetDevice(&dev));
+  SMELB_CHECK_ARG(dev < 64, kErrArg, "orthogonalize: device %d", dev);
+  if (raised[dev].load(std::memory_order_acquire) >= bytes) return kOk;
+  std::lock_guard<std::mutex> lk(mu);
+  if (raised[dev].load(std::memory_order_relaxed) < bytes) {
+    SMELB_CUDA(cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    raised[dev].store(bytes, std::memory_order_release);
+  }
+  return kOk;
+}
+
+template <auto KERN>
+int launch(const Args& a, long long blocks, int threads, long long smem, int cluster, cudaStream_t st) {
   SMELB_CHECK_ARG(blocks < (1LL << 31), kErrShape, "orthogonalize: %lld blocks", blocks);
-  SMELB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  if (int rc = raise_smem<KERN>(smem)) return rc;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)blocks);
   cfg.blockDim = dim3((unsigned)threads);
@@ -1080,7 +1100,7 @@ int launch(F* kern, const Args& a, long long blocks, int threads, long long smem
   at[0].val.clusterDim = {(unsigned)cluster, 1, 1};
   cfg.attrs = at;
   cfg.numAttrs = cluster > 1 ? 1 : 0;
-  SMELB_CUDA(cudaLaunchKernelEx(&cfg, kern, a));
+  SMELB_CUDA(cudaLaunchKernelEx(&cfg, KERN, a));
   count_launch();
   return kOk;
 }
@@ -1140,7 +1160,7 @@ int run_resident(Args& a, long long matrices, int maxL, cudaStream_t st) {
   }
   set_cap(a, cap);
   const long long smem = (long long)(D_::MAT + D_::work(c)) * 8 + (long long)NT * 8 * pitch(a.cap) * 4;
-  return launch(ortho_kernel<NT, T, MUON>, a, clusters * c, kThreads, smem, c, st);
+  return launch<ortho_kernel<NT, T, MUON>>(a, clusters * c, kThreads, smem, c, st);
 }
 
 template <int NT, typename T, bool MUON>
@@ -1154,11 +1174,11 @@ int run_split(Args& a, long long matrices, int maxL, double* ws, cudaStream_t st
     const long long n = std::min(kSplitRound, matrices - a.first);
     a.gram = ws;
     a.form = ws + n * blocks * D_::PART;
-    if (int rc = launch(gram_kernel<NT, T, MUON>, a, n * blocks, kThreads, (long long)D_::BUFS * D_::PART * 8 + x, 1, st))
+    if (int rc = launch<gram_kernel<NT, T, MUON>>(a, n * blocks, kThreads, (long long)D_::BUFS * D_::PART * 8 + x, 1, st))
       return rc;
-    if (int rc = launch(form_kernel<NT>, a, n, form_warps<NT>() * 32, (long long)(D_::MAT + D_::POLY) * 8, 1, st))
+    if (int rc = launch<form_kernel<NT>>(a, n, form_warps<NT>() * 32, (long long)(D_::MAT + D_::POLY) * 8, 1, st))
       return rc;
-    if (int rc = launch(product_kernel<NT, T, MUON>, a, n * blocks, kThreads, (long long)D_::MAT * 8 + x, 1, st))
+    if (int rc = launch<product_kernel<NT, T, MUON>>(a, n * blocks, kThreads, (long long)D_::MAT * 8 + x, 1, st))
       return rc;
   }
   return kOk;

@@ -1,5 +1,7 @@
 """Where the orthogonalised updates can go wrong besides their formulas: order within a block, host threads, polynomials that
 grow, small eps, overlapping tensors, captured optimizer steps. Bounds as in test_gpu_muon.py unless stated."""
+import threading
+
 import pytest
 import torch
 
@@ -23,3 +25,30 @@ def test_many_blocks_side_by_side_give_the_same_bits(dev, shape):
     check(first[::37], x[::37])
     for _ in range(20):
         assert torch.equal(smelb.orthogonalize(x), first)
+
+
+@pytest.mark.parametrize("rows", [24, 40])
+def test_host_threads_with_other_sizes(dev, rows):
+    """Threads that launch the same kernels with more and with less shared memory, each on its own stream: none is refused."""
+    import smelb
+    xs = [matrices(dev, (1, rows, n), "full", n) for n in (40, 500, 2000, 4000)]
+    want = [smelb.orthogonalize(x) for x in xs]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(k):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(300):
+                    out = smelb.orthogonalize(xs[k])
+                torch.cuda.current_stream().synchronize()
+                assert torch.equal(out, want[k])
+        except Exception as e:  # noqa: BLE001
+            failed.append((k, e))
+
+    threads = [threading.Thread(target=work, args=(k % 4,)) for k in range(8)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
