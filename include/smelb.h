@@ -450,6 +450,8 @@ int smelb_expert_usage(const float* probs, int64_t ld, const void* topv, int top
  * min(rows, cols) <= 64 (the width of a LoRA block): X = x / (|x|_F + eps), then `steps` (1..16) times
  * X <- a X + b (X X^T) X + c (X X^T)^2 X on the short side, with (a, b, c) = coefficients[3 s .. 3 s + 2] (host array) of
  * step s. out may alias x. dtype 0: fp32, 1: bf16 (x and out alike). Sums and products are fp64, the result is rounded once.
+ * Where the product of a^2 over the steps but the last passes 2^26 they are pairs of doubles (much slower): the rounding of
+ * fp64 grows by a^2 a step in directions that x barely has.
  * A matrix of zeros gives zeros; one that holds an infinity or NaN gives NaN and leaves the others alone. workspace:
  * 256-byte aligned, smelb_orthogonalize_workspace_bytes bytes (0 for short sides up to 32 unless they are very long). */
 int64_t smelb_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols);

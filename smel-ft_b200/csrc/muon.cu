@@ -12,6 +12,11 @@
 // the updates that allow it was built and was no faster (192 x 64 x 2048: 287 us against 278; 512 x 16 x 2048: 69, 66).
 // The momentum update itself is rounded to fp32, as its buffer is.
 //
+// The d x d recurrence never returns to x, so the rounding of G in directions that x barely has grows by a^2 a step: it moves the
+// result by up to 0.45 * 2^-53 times the product of the a^2 but the last (restated on the CPU against whole numbers of 260
+// bits). Polynomials that let the product pass 2^26 (more than eight steps of the usual one) take careful_kernel, which holds
+// sums and d x d matrices in pairs of doubles.
+//
 // Two ways, by the size of a matrix:
 //   resident  a cluster of 1 to 8 blocks holds one matrix in shared memory and reads it once (ortho_kernel)
 //   split     many blocks add partial Gram matrices of one matrix, one block forms P, many blocks apply it
@@ -634,13 +639,19 @@ __device__ __forceinline__ void load_row(const double* A, int i, double2 (&a)[NT
     a[k] = *reinterpret_cast<const double2*>(A + (i * NT + k) * 64 + 2 * (threadIdx.x & 31));
 }
 
-// Writes a tile and its mirror image.
-template <int NT>
+// Writes a tile and its mirror image. HALF: of a tile on the diagonal the upper half counts for both, as it must in G: S, a
+// polynomial of G G^T, then is symmetric by itself, while an asymmetry that only G's diagonal tiles keep would grow by more
+// than a^2 a step (eight steps on rank one: 3e-7 in the result, 6e-12 so).
+template <int NT, bool HALF = false>
 __device__ __forceinline__ void put_tile(double* M, const Spot<NT>& t, const double (&c)[2]) {
-  *reinterpret_cast<double2*>(M + t.own) = make_double2(c[0], c[1]);
+  if (!t.diagonal || !HALF) *reinterpret_cast<double2*>(M + t.own) = make_double2(c[0], c[1]);
   if (!t.diagonal) {
     M[t.mirror] = c[0];
     M[t.mirror + 8] = c[1];
+  } else if (HALF) {
+    const int lane = threadIdx.x & 31, r = lane >> 2, k = 2 * (lane & 3);
+    if (r <= k) M[t.own] = M[t.mirror] = c[0];
+    if (r <= k + 1) M[t.own + 1] = M[t.mirror + 8] = c[1];
   }
 }
 
@@ -778,7 +789,7 @@ __device__ double* iterate(const Args& a, double* G, double* work) {
           strip<NT, PARTS>(row, V, line, part, [&](const Spot<NT>& t, double (&c)[2]) {
             c[0] *= sc;
             c[1] *= sc;
-            put_tile<NT>(G, t, c);
+            put_tile<NT, true>(G, t, c);
           });
       } else {
 #pragma unroll
@@ -814,7 +825,7 @@ __device__ double* iterate(const Args& a, double* G, double* work) {
             product<NT>(S, V, chain[q], c);
             c[0] *= sc;
             c[1] *= sc;
-            put_tile<NT>(G, chain[q], c);
+            put_tile<NT, true>(G, chain[q], c);
           }
         }
       }
@@ -1055,6 +1066,198 @@ __global__ void __launch_bounds__(kThreads, NT >= 6 && !MUON && sizeof(T) == 4 ?
   }
 }
 
+// An unevaluated sum of two doubles, about 106 bits: Knuth's two-sum and the exact product by fma (intrinsics, which the
+// compiler does not contract).
+struct Pair {
+  double h, l;
+};
+__device__ __forceinline__ Pair two_sum(double a, double b) {
+  const double s = __dadd_rn(a, b), v = __dsub_rn(s, a);
+  return {s, __dadd_rn(__dsub_rn(a, __dsub_rn(s, v)), __dsub_rn(b, v))};
+}
+// c += a b, the low parts of the sum unnormalised.
+__device__ __forceinline__ void add_product(Pair& c, const Pair& a, const Pair& b) {
+  const double p = __dmul_rn(a.h, b.h);
+  const double e = __fma_rn(a.l, b.h, __fma_rn(a.h, b.l, __fma_rn(a.h, b.h, -p)));
+  const Pair s = two_sum(c.h, p);
+  c.h = s.h;
+  c.l = __dadd_rn(c.l, __dadd_rn(s.l, e));
+}
+// The same with an exact x (an fp32 value).
+__device__ __forceinline__ void add_product(Pair& c, const Pair& a, double x) {
+  const double p = __dmul_rn(a.h, x);
+  const Pair s = two_sum(c.h, p);
+  c.h = s.h;
+  c.l = __dadd_rn(c.l, __dadd_rn(s.l, __fma_rn(a.l, x, __fma_rn(a.h, x, -p))));
+}
+// c += p, exact.
+__device__ __forceinline__ void add(Pair& c, double p) {
+  const Pair s = two_sum(c.h, p);
+  c.h = s.h;
+  c.l = __dadd_rn(c.l, s.l);
+}
+__device__ __forceinline__ Pair times(const Pair& a, const Pair& b) {
+  Pair c{0.0, 0.0};
+  add_product(c, a, b);
+  return two_sum(c.h, c.l);
+}
+
+// A symmetric d x d matrix of pairs in shared memory, rows of an odd pitch.
+struct Wide {
+  double *h, *l;
+  int ld;
+  __device__ __forceinline__ Pair at(int i, int j) const { return {h[i * ld + j], l[i * ld + j]}; }
+  __device__ __forceinline__ void put(int i, int j, const Pair& v) const {
+    h[i * ld + j] = h[j * ld + i] = v.h;
+    l[i * ld + j] = l[j * ld + i] = v.l;
+  }
+};
+
+constexpr int kMaxPairs = kMaxD * (kMaxD + 1) / 2, kPairRounds = (kMaxPairs + kThreads - 1) / kThreads;
+
+// Columns [j0, j0 + w) into x [d][ld] element by element, in the order of memory.
+template <typename T, bool MUON>
+__device__ __forceinline__ void load_columns(const Args& a, const Tensor& t, long long base, int j0, int w, float* x, int ld,
+                                             bool first) {
+  for (int e = threadIdx.x; e < w * t.d; e += kThreads) {
+    const int c = t.tall ? e / t.d : e % w, i = t.tall ? e % t.d : e / w;
+    const long long at = base + (t.tall ? (long long)j0 * t.d + e : (long long)i * t.L + j0 + c);
+    float v = to_f(reinterpret_cast<const T*>(t.g)[at]);
+    if (MUON) {
+      float m = t.m[at];
+      v = update(a, v, m, first);
+      if (first) t.m[at] = m;
+    }
+    x[i * ld + c] = v;
+  }
+}
+
+// One block for one matrix, all of it in pairs of doubles: the Gram matrix (products of fp32 values are exact in fp64), the
+// steps, and P x, for which x is read a second time. A thread has up to nine elements of the upper triangle, or with few
+// rows a share of the columns of one. Bound by the fp64 units of the SM that has the matrix (a product and its sum take 8 to
+// 14 of their instructions, where the kernels above take one on the matrix units): 16 steps on 12 matrices of 16 x 2048
+// 0.37 ms, on 1548 of 16 x 1024 1.4, on 192 of 64 x 2048 8.7, on one of 64 x 40000 47. Polynomials this long are rare, so
+// the columns of a matrix are not spread over more blocks.
+template <typename T, bool MUON>
+__global__ void __launch_bounds__(kThreads) careful_kernel(const __grid_constant__ Args a) {
+  extern __shared__ __align__(16) double sm[];
+  const Tensor& t = tensor_of(a, blockIdx.x);
+  const long long base = ((long long)blockIdx.x - t.start) * t.d * t.L;
+  const int tid = threadIdx.x, d = t.d, pd = d | 1, count = d * (d + 1) / 2, ld = a.cap + 1;
+  const Wide G{sm, sm + d * pd, pd}, S{sm + 2 * d * pd, sm + 3 * d * pd, pd}, P{sm + 4 * d * pd, sm + 5 * d * pd, pd};
+  uint16_t* place = reinterpret_cast<uint16_t*>(sm + 6 * d * pd);  // (row, column) of each element of the upper triangle
+  float* x = reinterpret_cast<float*>(place + ((count + 7) & ~7));
+  for (int q = tid; q < d * d; q += kThreads) {
+    const int i = q / d, j = q - i * d;
+    if (j >= i) place[i * d - i * (i - 1) / 2 + j - i] = (uint16_t)(i << 8 | j);
+  }
+  const int groups = max(kThreads / count, 1), group = groups > 1 ? tid / count : 0;
+  Pair r[kPairRounds];
+#pragma unroll
+  for (int q = 0; q < kPairRounds; ++q) r[q] = {0.0, 0.0};
+  // calls f(element, its row, its column, r[q]) for the thread's elements
+  auto each = [&](auto&& f) {
+#pragma unroll
+    for (int q = 0; q < kPairRounds; ++q)
+      if (tid + q * kThreads < count) {
+        const int at = place[tid + q * kThreads];
+        f(at >> 8, at & 255, r[q]);
+      }
+  };
+  auto product = [&](const Wide& A, const Wide& B) {
+    each([&](int i, int j, Pair& c) {
+      c = {0.0, 0.0};
+      for (int k = 0; k < d; ++k) add_product(c, A.at(i, k), B.at(j, k));
+      c = two_sum(c.h, c.l);
+    });
+  };
+  auto write = [&](const Wide& M) {
+    each([&](int i, int j, const Pair& c) { M.put(i, j, c); });
+  };
+
+  for (int j0 = 0; j0 < t.L; j0 += a.cap) {
+    const int w = min(a.cap, t.L - j0);
+    load_columns<T, MUON>(a, t, base, j0, w, x, ld, true);
+    __syncthreads();
+    auto dot = [&](int i, int j, int c0, int step, Pair& s) {
+      for (int c = c0; c < w; c += step) add(s, __dmul_rn((double)x[i * ld + c], (double)x[j * ld + c]));
+    };
+    if (groups > 1) {
+      if (group < groups) {
+        const int at = place[tid - group * count];
+        dot(at >> 8, at & 255, group, groups, r[0]);
+      }
+    } else {
+      each([&](int i, int j, Pair& s) { dot(i, j, 0, 1, s); });
+    }
+    __syncthreads();
+  }
+  if (groups > 1) {
+    Pair* share = reinterpret_cast<Pair*>(x);
+    share[tid] = r[0];
+    __syncthreads();
+    if (tid < count)
+      for (int g = 1; g < groups; ++g) {
+        const Pair o = share[g * count + tid], s = two_sum(r[0].h, o.h);
+        r[0] = {s.h, r[0].l + (s.l + o.l)};
+      }
+  }
+  each([&](int i, int j, Pair& c) {
+    c = two_sum(c.h, c.l);
+    G.put(i, j, c);
+  });
+  __syncthreads();
+  double tr = 0.0;
+  for (int i = 0; i < d; ++i) tr += G.h[i * pd + i];
+  const double inv = tr == 0.0 ? 0.0 : 1.0 / (sqrt(tr) + a.eps), sq = __dmul_rn(inv, inv);
+  const Pair scale{sq, __fma_rn(inv, inv, -sq)};
+  __syncthreads();
+  each([&](int i, int j, Pair& c) { G.put(i, j, times(c, scale)); });
+  __syncthreads();
+  for (int step = 0; step < a.steps; ++step) {
+    const double ca = a.coef[step][0], cb = a.coef[step][1], cc = a.coef[step][2];
+    product(G, G);
+    each([&](int i, int j, const Pair& c) {  // S = a I + b G + c G^2
+      Pair s{i == j ? ca : 0.0, 0.0};
+      add_product(s, G.at(i, j), {cb, 0.0});
+      add_product(s, c, {cc, 0.0});
+      s = two_sum(s.h, s.l);
+      S.put(i, j, s);
+      if (step == 0) P.put(i, j, s);
+    });
+    __syncthreads();
+    if (step) {
+      product(S, P);
+      __syncthreads();
+      write(P);
+    }
+    if (step + 1 == a.steps) break;
+    product(S, G);
+    __syncthreads();
+    write(G);  // S G
+    __syncthreads();
+    product(S, G);
+    __syncthreads();
+    write(G);  // S G S
+    __syncthreads();
+  }
+  __syncthreads();
+
+  for (int j0 = 0; j0 < t.L; j0 += a.cap) {
+    const int w = min(a.cap, t.L - j0);
+    load_columns<T, MUON>(a, t, base, j0, w, x, ld, false);
+    __syncthreads();
+    for (int e = tid; e < w * d; e += kThreads) {
+      const int c = t.tall ? e / d : e % w, i = t.tall ? e % d : e / w;
+      Pair o{0.0, 0.0};
+      for (int k = 0; k < d; ++k) add_product(o, P.at(i, k), (double)x[k * ld + c]);
+      T* p = reinterpret_cast<T*>(t.p) + base + (t.tall ? (long long)j0 * d + e : (long long)i * t.L + j0 + c);
+      put(p, result<MUON>(a, t, (float)((o.h + o.l) * inv), MUON ? to_f(*p) : 0.f));
+    }
+    __syncthreads();
+  }
+}
+
 // Factor of a division of a number below 2^16 by n > 1: the high word of the product is the quotient.
 uint32_t by(int n) { return (uint32_t)((1ull << 32) / n + 1); }
 
@@ -1184,6 +1387,27 @@ int run_split(Args& a, long long matrices, int maxL, double* ws, cudaStream_t st
   return kOk;
 }
 
+// How much the rounding of G grows until the last step reads it, at most.
+double growth(int steps, const double* coef) {
+  double g = 1.0, most = 1.0;
+  for (int s = 0; s + 1 < steps; ++s) {
+    g = std::max(g, 1.0) * coef[3 * s] * coef[3 * s];
+    most = g > most || g != g ? g : most;
+  }
+  return most;
+}
+// Up to here 0.45 * 2^-53 * 2^26 is a twentieth of a rounding to fp32.
+constexpr double kMaxGrowth = 67108864.0;
+
+template <typename T, bool MUON>
+int run_careful(Args& a, int nt, long long matrices, cudaStream_t st) {
+  const int d = nt * 8;
+  a.cap = std::min(512, kMaxD * kMaxD / d / 32 * 32);
+  const long long x = std::max((long long)d * (a.cap + 1) * 4, (long long)kThreads * 16);
+  const long long smem = 6LL * d * (d | 1) * 8 + (d * (d + 1) / 2 + 7) / 8 * 16 + x;
+  return launch<careful_kernel<T, MUON>>(a, matrices, kThreads, smem, 1, st);
+}
+
 template <int NT, typename T, bool MUON>
 int run_way(Args& a, long long matrices, int maxL, bool held, double* ws, cudaStream_t st) {
   if constexpr (NT <= 4)
@@ -1286,6 +1510,7 @@ int run(const smelb_muon_tensor* t, int64_t n, int dtype, bool muon, double lr, 
   a.eps = eps;
   for (int s = 0; s < steps; ++s)
     for (int k = 0; k < 3; ++k) a.coef[s][k] = coef[3 * s + k];
+  const bool careful = !(growth(steps, coef) <= kMaxGrowth);
   return for_launches(t, n, [&](int nt, bool held, const int64_t* idx, int count, long long matrices, int maxL) {
     a.n = count;
     long long start = 0;
@@ -1299,6 +1524,10 @@ int run(const smelb_muon_tensor* t, int64_t n, int dtype, bool muon, double lr, 
       start += s.batch;
     }
     const bool bf = dtype == 1;
+    if (careful) {
+      if (muon) return bf ? run_careful<bf16, true>(a, nt, matrices, st) : run_careful<float, true>(a, nt, matrices, st);
+      return bf ? run_careful<bf16, false>(a, nt, matrices, st) : run_careful<float, false>(a, nt, matrices, st);
+    }
     double* w = (double*)ws;
     switch (nt) {
       case 1: return run_typed<1>(a, bf, muon, matrices, maxL, held, w, st);

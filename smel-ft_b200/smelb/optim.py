@@ -54,7 +54,9 @@ def orthogonalize(x, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
     """The Newton-Schulz polynomial of each matrix of x [..., m, n] (fp32 or bf16, min(m, n) <= 64): x / (|x|_F + eps), then
     `steps` (1..16) times X <- a X + b (X X^T) X + c (X X^T)^2 X on the short side. coefficients is (a, b, c), or one triple
     for each step. With the default ones the singular values end near 1. Returns a new tensor of x's shape and type; all
-    sums and products are fp64, the result is rounded once.
+    sums and products are fp64, the result is rounded once. Steps that would let the rounding of fp64 grow into the result
+    (the product of the a^2 but the last above 2^26: the default ones from the ninth on) are taken in pairs of doubles, which
+    is much slower.
 
     A matrix of zeros gives zeros; one with an infinity or NaN gives NaN and leaves the others alone. There is no
     gradient: x must not require one unless gradients are off."""

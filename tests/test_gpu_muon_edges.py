@@ -1,11 +1,14 @@
 """Where the orthogonalised updates can go wrong besides their formulas: order within a block, host threads, polynomials that
 grow, small eps, overlapping tensors, captured optimizer steps. Bounds as in test_gpu_muon.py unless stated."""
+import math
 import threading
+from fractions import Fraction
 
+import numpy as np
 import pytest
 import torch
 
-from test_gpu_muon import check, matrices
+from test_gpu_muon import COEF, U, check, check_step, matrices, tensors
 
 pytestmark = pytest.mark.gpu
 
@@ -52,3 +55,90 @@ def test_host_threads_with_other_sizes(dev, rows):
     for t in threads:
         t.join()
     assert not failed, failed
+
+
+def truth(x, steps, coef=COEF, eps=1e-7, bits=260):
+    """The iteration on x in whole numbers of 2^-bits: what 64 bits cannot hold once small singular values have grown."""
+    if x.dim() > 2:
+        return torch.stack([truth(m, steps, coef, eps, bits) for m in x])
+    if x.shape[0] > x.shape[1]:
+        return truth(x.mT, steps, coef, eps, bits).mT
+    fix = lambda v: int(Fraction(float(v)) * (1 << bits))  # noqa: E731
+    X = np.array([[fix(v) for v in row] for row in x.double().cpu().tolist()], dtype=object)
+    n = math.isqrt(int((X * X).sum())) + fix(eps)
+    X = (X << bits) // n
+    for a, b, c in [coef] * steps if np.ndim(coef) == 1 else coef:
+        G = X @ X.T >> bits
+        S = fix(b) * G + (fix(c) * (G @ G >> bits)) >> bits
+        S[np.diag_indices(len(S))] += fix(a)
+        X = S @ X >> bits
+    return torch.tensor([[float(Fraction(int(v), 1 << bits)) for v in row] for row in X], dtype=torch.float64)
+
+
+def check_grown(out, x, steps, coef=COEF):
+    """One rounding of the result, 1e-9 for the sums, and 2^-53 * 2^26 for a rounding of G that has grown as far as the kernels in
+    single doubles let it (the result's singular values are at most 1.3)."""
+    ref = truth(x, steps, coef)
+    rms = ref.pow(2).mean((-1, -2), keepdim=True).sqrt()
+    tol = U * ref.abs() + 1e-9 * rms + 2.0 ** -27
+    if x.dtype == torch.bfloat16:
+        tol = tol + 2.0 ** -8 * (ref.abs() + tol)
+    err = (out.double().cpu() - ref).abs()
+    assert bool((err <= tol).all()), f"{tuple(x.shape)}, {steps} steps: {(err / tol).max().item():.2f} of the bound"
+
+
+@pytest.mark.parametrize("steps", [7, 8, 10, 12, 14, 16])
+@pytest.mark.parametrize("m,n", [(16, 96), (96, 16), (5, 40), (1, 9), (24, 60), (33, 70), (100, 64), (3, 4200)])
+def test_many_steps_on_matrices_of_low_rank(dev, m, n, steps):
+    """Singular values near zero, as gradients of few tokens have, grow by 3.4 a step: to one after 16 of fp32's rounding."""
+    import smelb
+    for dtype in (torch.float32, torch.bfloat16):
+        kinds = ("rank1", "rank3", "decay") if m * n < 3000 else ("rank1",)
+        x = torch.stack([matrices(dev, (m, n), kind, steps + m) for kind in kinds] + [torch.zeros(m, n, device=dev)]).to(dtype)
+        out = smelb.orthogonalize(x, steps=steps)
+        check_grown(out, x, steps)
+        assert not out[-1].any() and torch.equal(out, smelb.orthogonalize(x, steps=steps))
+
+
+def test_growth_is_what_counts(dev):
+    """Triples of their own for each step, large ones first, and many steps that grow little."""
+    import smelb
+    coef = ((8.28721, -23.5959, 17.30039), (4.10706, -2.94785, 0.54484), (3.94869, -2.90890, 0.55182), (3.31842, -2.48849, 0.51005),
+            (2.30065, -1.66890, 0.41888), (1.89130, -1.26800, 0.37680), (1.875, -1.25, 0.375), (1.875, -1.25, 0.375),
+            (1.875, -1.25, 0.375), (1.875, -1.25, 0.375))
+    for shape in ((2, 16, 60), (2, 40, 50)):
+        for kind in ("rank1", "decay"):
+            x = matrices(dev, shape, kind, 3)
+            for steps in (8, 10):
+                check_grown(smelb.orthogonalize(x, steps=steps, coefficients=coef[:steps]), x, steps, coef[:steps])
+            check_grown(smelb.orthogonalize(x, steps=16, coefficients=(1.875, -1.25, 0.375)), x, 16, (1.875, -1.25, 0.375))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("nesterov", [False, True])
+def test_muon_step_of_many_steps(dev, dtype, nesterov):
+    """Full-rank updates, which the 64-bit singular values still settle, of every size class in one step."""
+    import smelb
+    shapes = [(3, 16, 128), (3, 128, 16), (1, 1), (8, 8), (2, 600, 24), (40, 90), (64, 64), (2, 7, 5000), (0, 16, 32), (1, 30)]
+    params, grads, bufs = tensors(dev, shapes, 13, dtype)
+    grads, bufs = [torch.randn_like(g) * 1e-3 for g in grads], [torch.randn_like(m) * 1e-3 for m in bufs]
+    before = [(p.clone(), m.clone()) for p, m in zip(params, bufs)]
+    smelb.muon_step(params, grads, bufs, lr=0.02, nesterov=nesterov, weight_decay=0.1, steps=12)
+    check_step(before, params, grads, bufs, 0.02, nesterov=nesterov, wd=0.1, steps=12)
+
+
+def test_many_steps_strides_values_and_aliasing(dev):
+    import smelb
+    base = matrices(dev, (4, 40, 300), "full", 3)
+    for x in (base[:, :16], base[:, ::3, 1:258], base[:, :16].mT, base.reshape(-1)[1:1 + 3 * 16 * 200].view(3, 16, 200)):
+        assert torch.equal(smelb.orthogonalize(x, steps=10), smelb.orthogonalize(x.contiguous().clone(), steps=10))
+        check(smelb.orthogonalize(x, steps=10), x, steps=10)
+    x = matrices(dev, (6, 16, 100), "full", 2)
+    want = smelb.orthogonalize(x, steps=10)
+    x[1, 3, 7], x[4, 0, 99] = float("nan"), float("inf")
+    out = smelb.orthogonalize(x, steps=10)
+    assert out[1].isnan().all() and out[4].isnan().all()
+    assert all(torch.equal(out[i], want[i]) for i in (0, 2, 3, 5))
+    for scale in (1e-44, 1e-8, 1e30):
+        y = matrices(dev, (2, 16, 60), "full", 5) * scale
+        check(smelb.orthogonalize(y, steps=9), y, steps=9)
