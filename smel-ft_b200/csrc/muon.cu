@@ -739,7 +739,7 @@ __device__ double* iterate(const Args& a, double* G, double* work) {
   for (int i = NT <= 2 ? lane % D_::D : lane; i < D_::D; i += 32) tr += G[(i >> 3) * (NT + 1) * 64 + (i & 7) * 9];
 #pragma unroll
   for (int o = NT == 1 ? 4 : NT == 2 ? 8 : 16; o; o >>= 1) tr += __shfl_xor_sync(0xffffffffu, tr, o);
-  const double inv = 1.0 / (sqrt(tr) + a.eps);
+  const double inv = tr == 0.0 ? 0.0 : 1.0 / (sqrt(tr) + a.eps);  // zeros stay zeros however small eps is
   if constexpr (2 * NT * NT <= WARPS) {
     __syncthreads();  // every warp has its trace: the chain overwrites G without waiting for the others
     iterate_small<NT>(a, G, work, inv);

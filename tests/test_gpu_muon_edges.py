@@ -142,3 +142,20 @@ def test_many_steps_strides_values_and_aliasing(dev):
     for scale in (1e-44, 1e-8, 1e30):
         y = matrices(dev, (2, 16, 60), "full", 5) * scale
         check(smelb.orthogonalize(y, steps=9), y, steps=9)
+
+
+@pytest.mark.parametrize("eps", [1e-80, 1e-300])
+def test_zeros_stay_zeros_with_any_eps(dev, eps):
+    """1 / eps^4 is past fp64 here; matrices of fp32's smallest numbers are orthogonalised as any other."""
+    import smelb
+    for m, n in ((4, 9), (8, 40), (16, 300), (30, 24), (100, 40), (64, 2048), (16, 5000)):
+        for steps in (5, 10):
+            x = matrices(dev, (4, m, n), "full", m)
+            x[1], x[2] = 0.0, x[2] * 1e-43
+            out = smelb.orthogonalize(x, eps=eps, steps=steps)
+            assert not out[1].any()
+            check(out[::2], x[::2], eps=eps, steps=steps)
+    p = [torch.ones(3, 16, 64, device=dev), torch.ones(2, 64, 40, device=dev)]
+    zeros = [torch.zeros_like(t) for t in p]
+    smelb.muon_step(p, zeros, [z.clone() for z in zeros], lr=0.1, eps=eps)
+    assert all(bool((t == 1).all()) for t in p)
