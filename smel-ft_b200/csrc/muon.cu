@@ -840,8 +840,22 @@ __device__ double* iterate(const Args& a, double* G, double* work) {
   return P;
 }
 
+// fp64 to fp32, to nearest. ODD: towards zero with the last bit set if anything was cut off, so that a later rounding to bf16
+// (16 bits fewer) is the only one.
+template <bool ODD>
+__device__ __forceinline__ float narrow(double v) {
+  if constexpr (!ODD) return (float)v;
+  const float f = __double2float_rz(v);
+  return (double)f != v ? __uint_as_float(__float_as_uint(f) | 1u) : f;
+}
+// Whether a result of type T goes through fp32 on its way to bf16. The Muon step's goes into an fp32 sum first.
+template <typename T, bool MUON>
+constexpr bool odd() {
+  return !MUON && sizeof(T) == 2;
+}
+
 // x <- P x in place in fp64: a warp owns C groups of eight columns at a time. Up to 16 rows P stays in registers.
-template <int NT>
+template <int NT, bool ODD>
 __device__ __forceinline__ void apply(const double* P, float* x, int ld, int w) {
   constexpr int C = NT <= 4 ? 2 : 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
@@ -886,7 +900,7 @@ __device__ __forceinline__ void apply(const double* P, float* x, int ld, int w) 
 #pragma unroll
         for (int i = 0; i < NT; ++i)
           *reinterpret_cast<float2*>(x + (8 * i + r) * ld + j + g * kWarps * 8 + 2 * c) =
-              make_float2((float)o[g][i][0], (float)o[g][i][1]);
+              make_float2(narrow<ODD>(o[g][i][0]), narrow<ODD>(o[g][i][1]));
       }
   }
 }
@@ -974,7 +988,7 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 ? 4 : 2) ortho_kernel(const 
     return;
   }
   const double* P = iterate<NT, kWarps>(a, G, work);
-  apply<NT>(P, x, ld, w);
+  apply<NT, odd<T, MUON>()>(P, x, ld, w);
   __syncthreads();
   if (w) store_slice<T, MUON>(a, t, base, j0, w, x, ld);
   if (a.blocks > 1) cluster_wait();
@@ -1059,7 +1073,7 @@ __global__ void __launch_bounds__(kThreads, NT >= 6 && !MUON && sizeof(T) == 4 ?
     const int w = min(a.cap, t.L - j0);
     load_slice<NT, T, MUON>(a, t, base, j0, w, x, ld, false);
     __syncthreads();
-    apply<NT>(sm, x, ld, w);
+    apply<NT, odd<T, MUON>()>(sm, x, ld, w);
     __syncthreads();
     store_slice<T, MUON>(a, t, base, j0, w, x, ld);
     __syncthreads();
@@ -1252,7 +1266,7 @@ __global__ void __launch_bounds__(kThreads) careful_kernel(const __grid_constant
       Pair o{0.0, 0.0};
       for (int k = 0; k < d; ++k) add_product(o, P.at(i, k), (double)x[k * ld + c]);
       T* p = reinterpret_cast<T*>(t.p) + base + (t.tall ? (long long)j0 * d + e : (long long)i * t.L + j0 + c);
-      put(p, result<MUON>(a, t, (float)((o.h + o.l) * inv), MUON ? to_f(*p) : 0.f));
+      put(p, result<MUON>(a, t, narrow<odd<T, MUON>()>((o.h + o.l) * inv), MUON ? to_f(*p) : 0.f));
     }
     __syncthreads();
   }

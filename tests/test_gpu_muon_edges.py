@@ -159,3 +159,22 @@ def test_zeros_stay_zeros_with_any_eps(dev, eps):
     zeros = [torch.zeros_like(t) for t in p]
     smelb.muon_step(p, zeros, [z.clone() for z in zeros], lr=0.1, eps=eps)
     assert all(bool((t == 1).all()) for t in p)
+
+
+@pytest.mark.parametrize("shape", [(3000, 16, 96), (3000, 96, 13), (600, 30, 200), (300, 64, 240), (40, 16, 5000)])
+def test_bf16_results_are_rounded_once(dev, shape):
+    """Next to the middle between two bf16 numbers a rounding to fp32 on the way would decide wrongly: none may be more than
+    half a step off (but for 1e-9, what the sums in 64 bits may be off)."""
+    import smelb
+    x = matrices(dev, shape, "full", 8).bfloat16()
+    X = x.double() if shape[1] <= shape[2] else x.double().mT  # the iteration itself, on the device for its size
+    X = X / (X.square().sum((-1, -2), keepdim=True).sqrt() + 1e-7)
+    a, b, c = COEF
+    for _ in range(5):
+        G = X @ X.mT
+        X = a * X + (b * G + c * G @ G) @ X
+    ref = X if shape[1] <= shape[2] else X.mT
+    out = smelb.orthogonalize(x).double()
+    step = torch.exp2(torch.floor(torch.log2(ref.abs())) - 7)  # bf16 keeps seven bits behind the first
+    err = (out - ref).abs()
+    assert ref.numel() > 3e6 and bool((err <= step / 2 + 1e-9 * step).all()), (err / step).max().item()
