@@ -449,7 +449,7 @@ int smelb_expert_usage(const float* probs, int64_t ld, const void* topv, int top
  * No counterpart in the reference (it trains its LoRA factors with AdamW). For each [rows, cols] matrix x of a batch,
  * min(rows, cols) <= 64 (the width of a LoRA block): X = x / (|x|_F + eps), then `steps` (1..16) times
  * X <- a X + b (X X^T) X + c (X X^T)^2 X on the short side, with (a, b, c) = coefficients[3 s .. 3 s + 2] (host array) of
- * step s. out may alias x. dtype 0: fp32, 1: bf16 (x and out alike). Sums and products are fp64, the result is rounded once.
+ * step s. out may be x, else they must not overlap. dtype 0: fp32, 1: bf16 (x and out alike). Sums and products are fp64, the result is rounded once.
  * Where the product of a^2 over the steps but the last passes 2^26 they are pairs of doubles (much slower): the rounding of
  * fp64 grows by a^2 a step in directions that x barely has.
  * A matrix of zeros gives zeros; one that holds an infinity or NaN gives NaN and leaves the others alone. workspace:
@@ -463,7 +463,7 @@ int smelb_orthogonalize(const void* x, int dtype, int64_t batch, int64_t rows, i
  *   m <- momentum m + (1 - momentum) g;  u = nesterov ? momentum m + (1 - momentum) g : m
  *   p <- p (1 - lr weight_decay) - lr f orthogonalize(u),  f = sqrt(max(1, rows / cols)) (adjust 0) or
  *   0.2 sqrt(max(rows, cols)) (adjust 1).
- * p and g of the dtype (0: fp32, 1: bf16), m fp32. No tensor may overlap another. workspace: 256-byte aligned,
+ * p and g of the dtype (0: fp32, 1: bf16), m fp32. A p or m that overlaps another tensor is refused. workspace: 256-byte aligned,
  * smelb_muon_workspace_bytes bytes (it reads the tensors' sizes alone; -1 for sizes that are refused). */
 typedef struct smelb_muon_tensor {
   void* p;

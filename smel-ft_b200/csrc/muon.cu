@@ -23,7 +23,9 @@
 //             (gram_kernel, form_kernel, product_kernel); x is read twice
 #include <algorithm>
 #include <atomic>
+#include <memory>
 #include <mutex>
+#include <new>
 
 #include "common.cuh"
 #include "host.h"
@@ -1496,6 +1498,37 @@ long long workspace(const smelb_muon_tensor* t, int64_t n) {
   return most;
 }
 
+// Refuses tensors of which one that is written shares memory with another (out of an orthogonalisation may be x itself).
+int check_overlap(const smelb_muon_tensor* t, int64_t n, int bytes, bool muon, const char* what) {
+  struct Span {
+    uintptr_t lo, hi;
+    int64_t tensor;
+    bool written;
+  };
+  std::unique_ptr<Span[]> spans(new (std::nothrow) Span[(size_t)n * 3]);
+  SMELB_CHECK_ARG(spans || n == 0, kErrArg, "%s: no host memory for %lld tensors", what, (long long)n);
+  int64_t count = 0;
+  for (int64_t i = 0; i < n; ++i) {
+    const uintptr_t e = (uintptr_t)(t[i].batch * t[i].rows * t[i].cols);
+    auto span = [&](const void* at, int size, bool written) {
+      if (e) spans[count++] = {(uintptr_t)at, (uintptr_t)at + e * size, i, written};
+    };
+    span(t[i].p, bytes, true);
+    if (muon || t[i].g != t[i].p) span(t[i].g, bytes, false);
+    if (muon) span(t[i].m, 4, true);
+  }
+  std::sort(spans.get(), spans.get() + count, [](const Span& a, const Span& b) { return a.lo < b.lo; });
+  const Span *any = nullptr, *out = nullptr;  // those that reach farthest so far, of all and of the written ones
+  for (const Span* s = spans.get(); s < spans.get() + count; ++s) {
+    const Span* hit = s->written ? any : out;
+    SMELB_CHECK_ARG(!hit || hit->hi <= s->lo, kErrArg, "%s: tensors %lld and %lld share memory that is written", what,
+                    (long long)hit->tensor, (long long)s->tensor);
+    if (!any || s->hi > any->hi) any = s;
+    if (s->written && (!out || s->hi > out->hi)) out = s;
+  }
+  return kOk;
+}
+
 int run(const smelb_muon_tensor* t, int64_t n, int dtype, bool muon, double lr, double mu, bool nesterov, double wd,
         int adjust, int steps, const double* coef, double eps, void* ws, int64_t ws_bytes, const char* what,
         cudaStream_t st) {
@@ -1505,6 +1538,7 @@ int run(const smelb_muon_tensor* t, int64_t n, int dtype, bool muon, double lr, 
   SMELB_CHECK_ARG(dtype == 0 || dtype == 1, kErrDtype, "%s: dtype %d", what, dtype);
   SMELB_CHECK_ARG(steps >= 1 && steps <= kMaxSteps && coef, kErrArg, "%s: %d steps (1..%d)", what, steps, kMaxSteps);
   SMELB_CHECK_ARG(eps > 0.0, kErrArg, "%s: eps must be positive", what);
+  if (int rc = check_overlap(t, n, dtype == 1 ? 2 : 4, muon, what)) return rc;
   const long long need = workspace(t, n);
   SMELB_CHECK_ARG(ws_bytes >= need && (ws || !need), kErrWorkspace, "%s: workspace %lld bytes, %lld needed", what,
                   (long long)ws_bytes, need);

@@ -86,8 +86,9 @@ def muon_step(params, grads, buffers, lr, momentum=0.95, nesterov=True, weight_d
 
     for every [m, n] matrix of a tensor, f = sqrt(max(1, m / n)) ("original") or 0.2 sqrt(max(m, n)) ("match_rms_adamw").
     params: contiguous fp32 or bf16 [..., m, n], min(m, n) <= 64, all of one type and device; grads alike; buffers: contiguous
-    fp32 of the params' shapes. No two of the tensors written may overlap. One kernel launch takes up to 48 tensors whose
-    short sides round up to the same multiple of 8 (short sides above 32, and very long matrices, take three)."""
+    fp32 of the params' shapes. A param or buffer that shares memory with another tensor is refused. One kernel launch takes
+    up to 48 tensors whose short sides round up to the same multiple of 8 (short sides above 32, and very long matrices, take
+    three)."""
     who = "muon_step"
     params, grads, buffers = list(params), list(grads), list(buffers)
     if not len(params) == len(grads) == len(buffers):

@@ -137,3 +137,37 @@ def test_workspace_sizes():
         t[i].batch, t[i].rows, t[i].cols = b, m, n
     assert lib.smelb_muon_workspace_bytes(t, 2) == max(ws(3, 64, 500), ws(7, 2000, 48))
     assert lib.smelb_muon_workspace_bytes(t, 0) == 0 and lib.smelb_muon_workspace_bytes(None, 0) == 0
+
+
+def test_overlapping_tensors_are_refused():
+    """A tensor that is written may share memory with no other one, whole or in part; gradients may with each other."""
+    from smelb import _lib
+    lib = _lib.load()
+    coef = (ctypes.c_double * 15)(*([1.0, 0.0, 0.0] * 5))
+    size, at = 16 * 32 * 4, 1 << 20  # the addresses are never used: a check fails first
+
+    def step(*tensors, dtype=0):
+        t = (_lib.MuonTensor * len(tensors))()
+        for i, (p, g, m, batch) in enumerate(tensors):
+            t[i].p, t[i].g, t[i].m, t[i].batch, t[i].rows, t[i].cols = at + p, at + g, at + m, batch, 16, 32
+        # the last check before the launches wants a 256-byte aligned workspace: -6 with this text is "no overlap found"
+        rc = lib.smelb_muon_step(t, len(tensors), dtype, 0.1, 0.9, 1, 0.0, 0, 5, coef, 1e-7, 8, 0, None)
+        return rc, _lib.last_error()
+
+    fine = (-6, "aligned")
+    for tensors, dtype, want in (
+            (((0, size, 2 * size, 1),), 0, fine),
+            (((0, size, 2 * size, 1), (3 * size, size, 4 * size, 1)), 0, fine),             # one gradient for two
+            (((0, size, 2 * size, 1), (3 * size, size + 64, 4 * size, 1)), 0, (-6, "share")),   # it reaches into a buffer
+            (((0, size // 2, size, 1),), 1, fine),                                            # bf16: half the bytes
+            (((0, size // 2, size, 1),), 0, (-6, "share")),
+            (((4, size + 4, size, 1),), 0, (-6, "share")),
+            (((0, size, 2 * size, 2),), 0, (-6, "share")),                                    # a longer batch
+            (((0, 9 * size, 2 * size, 2), (4 * size, 5 * size, size - 4, 1)), 0, (-6, "share")),
+            (((0, 0, 0, 0), (0, size, 2 * size, 1)), 0, fine),                                # an empty one anywhere
+            (((10 * size, 0, 20 * size, 8), (9 * size, 30 * size, 17 * size - 4, 1)), 0, (-6, "share"))):
+        rc, text = step(*tensors, dtype=dtype)
+        assert rc == want[0] and want[1] in text, (tensors, rc, text)
+    o = lambda x, out: lib.smelb_orthogonalize(at + x, 0, 1, 16, 32, 5, coef, 1e-7, at + out, 8, 0, None)  # noqa: E731
+    for x, out, text in ((0, 0, "aligned"), (0, size, "aligned"), (0, 4, "share"), (size - 4, 0, "share")):
+        assert o(x, out) == -6 and text in _lib.last_error(), (x, out)
