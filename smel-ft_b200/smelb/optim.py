@@ -151,7 +151,8 @@ def _refuse(who, i, p, g, m, dtype, dev):
 class Muon(torch.optim.Optimizer):
     """muon_step as a torch optimizer over parameters [..., m, n] with min(m, n) <= 64 (the factors of ExpertsLoRA and
     MLPLoRA). State per parameter: momentum_buffer, fp32 of the parameter's shape. A parameter without a gradient is
-    left alone. lr may change between steps (a scheduler's); a captured step keeps the lr it was captured with."""
+    left alone. lr may change between steps (a scheduler's); a captured step keeps the lr it was captured with. The step
+    that makes a parameter's state cannot be captured."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, adjust="original", steps=5,
                  coefficients=COEFFICIENTS, eps=1e-7):
@@ -193,6 +194,8 @@ class Muon(torch.optim.Optimizer):
                     continue
                 state = self.state[p]
                 if "momentum_buffer" not in state:
+                    if p.is_cuda and torch.cuda.is_current_stream_capturing():  # each replay would fill it with zeros again
+                        raise _lib.SmelbError("Muon: take a step before one is captured (it makes the momentum buffers)")
                     state["momentum_buffer"] = torch.zeros_like(p, dtype=torch.float32,
                                                                 memory_format=torch.contiguous_format)
                 by_kind.setdefault((p.device, p.dtype), []).append((p, p.grad, state["momentum_buffer"]))

@@ -178,3 +178,28 @@ def test_bf16_results_are_rounded_once(dev, shape):
     step = torch.exp2(torch.floor(torch.log2(ref.abs())) - 7)  # bf16 keeps seven bits behind the first
     err = (out - ref).abs()
     assert ref.numel() > 3e6 and bool((err <= step / 2 + 1e-9 * step).all()), (err / step).max().item()
+
+
+def test_captured_optimizer_steps_keep_their_momentum(dev):
+    """A captured first step would make new buffers of zeros at each replay: it is refused, and after one step in the open the
+    replays are the steps."""
+    import smelb
+    params, grads, _ = tensors(dev, [(3, 16, 128), (96, 16), (64, 40)], 17)
+    ps, qs = ([torch.nn.Parameter(p.clone()) for p in params] for _ in range(2))
+    opt, ref = smelb.Muon(ps, lr=0.05), smelb.Muon(qs, lr=0.05)
+    for p, q, g in zip(ps, qs, grads):
+        p.grad, q.grad = g.clone(), g.clone()
+    with pytest.raises(smelb.SmelbError, match="take a step before"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.step()
+    assert all(torch.equal(p, q) for p, q in zip(ps, qs))
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    ref.step()
+    for _ in range(3):
+        graph.replay()
+        ref.step()
+    assert all(torch.equal(p, q) for p, q in zip(ps, qs))
+    assert all(torch.equal(opt.state[p]["momentum_buffer"], ref.state[q]["momentum_buffer"]) for p, q in zip(ps, qs))
