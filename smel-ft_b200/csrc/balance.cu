@@ -522,7 +522,7 @@ Layout layout(long long T, long long E, long long S, bool usage) {
   Layout l{};
   l.rows = tile_rows(T);
   l.tiles = (int)((T + l.rows - 1) / l.rows);
-  l.cols = S > 16 && l.tiles < 4 * S ? 0 : S * E < 32 * 148 ? 8 : 32;
+  l.cols = usage ? 8 : S > 16 && l.tiles < 4 * S ? 0 : S * E < 32 * 148 ? 8 : 32;
   const long long recs = l.tiles + S, eb = (E + 31) / 32 * (l.cols == 8 ? 4 : 1);
   long long o = 0;
   auto take = [&](long long bytes) {
@@ -568,12 +568,15 @@ int run_tiles(const TileArgs& t, int tiles, cudaStream_t st) {
 template <bool USAGE>
 int run_finish(const FinArgs& f, int cols, cudaStream_t st) {
   const dim3 grid((unsigned)f.S, (unsigned)((f.E + std::max(cols, 1) - 1) / std::max(cols, 1)));
-  if (cols == 0) {
+  if (USAGE || cols == 8) {
+    balance_finish_kernel<USAGE, 8><<<grid, kFinThreads, 0, st>>>(f);
+  } else if (cols == 32) {
+    balance_finish_kernel<false, 32><<<grid, kFinThreads, 0, st>>>(f);
+  } else {
     const int per = kFinThreads / 32;
     balance_finish_short_kernel<<<dim3((unsigned)((f.S + per - 1) / per), (unsigned)((f.E + 31) / 32)), kFinThreads, 0,
                                   st>>>(f);
-  } else if (cols == 8) balance_finish_kernel<USAGE, 8><<<grid, kFinThreads, 0, st>>>(f);
-  else balance_finish_kernel<USAGE, 32><<<grid, kFinThreads, 0, st>>>(f);
+  }
   SMELB_CUDA(cudaGetLastError());
   count_launch();
   return kOk;
