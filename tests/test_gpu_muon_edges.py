@@ -203,3 +203,21 @@ def test_captured_optimizer_steps_keep_their_momentum(dev):
         ref.step()
     assert all(torch.equal(p, q) for p, q in zip(ps, qs))
     assert all(torch.equal(opt.state[p]["momentum_buffer"], ref.state[q]["momentum_buffer"]) for p, q in zip(ps, qs))
+
+
+def test_bf16_results_below_the_normal_numbers(dev):
+    """Multiples of 2^-133 are bf16's numbers there."""
+    import smelb
+    x = torch.randn(2000, 1, 60, generator=torch.Generator(device=dev).manual_seed(4), device=dev).bfloat16()
+    x[:, 0, 1:] *= torch.exp2(torch.randint(-134, -120, (2000, 59), device=dev).float()).bfloat16()
+    X = x.double()
+    t = X.square().sum((-1, -2), keepdim=True).sqrt()
+    s = t / (t + 1e-7)
+    a, b, c = COEF
+    r = s.clone()
+    for _ in range(5):
+        r = r * (a + b * r ** 2 + c * r ** 4)
+    ref = X / t * r
+    step = torch.exp2(torch.floor(torch.log2(ref.abs())).clamp(min=-126) - 7)
+    err = (smelb.orthogonalize(x).double() - ref).abs()
+    assert bool((err[ref != 0] <= (step / 2 * (1 + 1e-9))[ref != 0]).all()) and bool((err[ref == 0] == 0).all())
