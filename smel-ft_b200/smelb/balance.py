@@ -11,7 +11,10 @@ In a training step:
     out = smelb.moe_forward(x, W, ex, top_k, lora, stats=lambda p, v, i: aux.append(smelb.balance_loss(p, i)[0]))
     (task_loss(out) + 0.01 * aux[0]).backward()
 
-probs is differentiable there, so the loss reaches x through the layer's own router backward.
+probs is differentiable there, so the loss reaches x through the layer's own router backward. The router's weight is frozen
+and gets no gradient: the loss trains what lies below the layer. moe_block_gemma4 and moe_forward_ep take the same callback (with
+moe_forward_ep each rank's loss is of its own tokens). LayerMajorRunner calls it in its forward alone, which keeps no graph: there
+the loss and the usage are figures to watch.
 """
 import torch
 
