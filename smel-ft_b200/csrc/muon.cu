@@ -9,7 +9,7 @@
 // G moves the result by delta / sigma^2, so gradients of low rank (few tokens reached the expert) come out up to 3e-4
 // off when G is held in fp32, and 6e-5 with the last product alone in fp32 (P has entries up to 485 there, and the sums
 // cancel them). All of it is fp64, on the fp64 matrix instruction (m8n8k4), and rounded once. An fp32 last product for
-// the updates that allow it was built and was no faster (192 x 64 x 2048: 287 us against 278; 512 x 16 x 2048: 69, 66).
+// the updates that allow it was built and was no faster (192 x 64 x 2048: 287 us against 275; 512 x 16 x 2048: 69, 64).
 // The momentum update itself is rounded to fp32, as its buffer is.
 //
 // The d x d recurrence never returns to x, so the rounding of G in directions that x barely has grows by a^2 a step: it moves the
@@ -923,7 +923,7 @@ __device__ __forceinline__ const Tensor& tensor_of(const Args& a, long long at) 
 // Resident: the blocks of a cluster hold one matrix, or a few short ones, `cap` columns each at most. Their parts of the
 // Gram matrix go to every block of the matrix by asynchronous stores into its shared memory that the receiver's barrier
 // counts: one way, and without the fence over the stores to the momentum buffer that a cluster barrier would need.
-// Bound: one matrix at a time by latency (7.0 us for 12 matrices of 16 x 2048: of 13000 cycles 4100 the polynomial, 1650
+// Bound: one matrix at a time by latency (7.5 us for 12 matrices of 16 x 2048: of 13000 cycles 4100 the polynomial, 1650
 // the last product, 1150 the loads); many by HBM and the fp64 units together (a Muon step of 1548 matrices of rank 16,
 // 634 MB: 142 us, 4.5 TB/s, the units half busy; loads and stores alone take 106).
 template <int NT, typename T, bool MUON>
@@ -999,8 +999,8 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 ? 4 : 2) ortho_kernel(const 
 }
 
 // Split: block b of a matrix takes the chunks b, b + blocks, ... of `cap` columns. Bound by the fp64 units: 192 x 64 x 2048
-// in 82 us, 49 at their rate; three blocks to an SM where the registers allow it, as two (94 us) leave the units idle
-// while a block loads.
+// in 82 us, 49 at their rate (here and below a kernel alone with cold caches; a pass of the three takes 277); three blocks to
+// an SM where the registers allow it, as two (94 us) leave the units idle while a block loads.
 template <int NT, typename T, bool MUON>
 __global__ void __launch_bounds__(kThreads, NT == 6 || MUON || sizeof(T) == 2 ? 2 : 3)
     gram_kernel(const __grid_constant__ Args a) {
@@ -1332,7 +1332,7 @@ constexpr int kMaxBlocks = 8;
 constexpr int kBlockCols = 512;
 
 // Whether matrices of this size are held by a cluster: up to 32 rows, and no more columns than eight blocks hold (1548
-// matrices of rank 16 the split way: 236 us a step against 144; 512 x 16 x 2048: 85 against 69).
+// matrices of rank 16 the split way: 225 us a step against 142; 512 x 16 x 2048: 80 against 64).
 bool resident(int nt, int L) { return nt <= 4 && L <= kBlockCols * kMaxBlocks; }
 
 // Blocks that a resident matrix needs.
